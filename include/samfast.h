@@ -239,6 +239,51 @@ int samfast_linear_half(
     int64_t M, int N, int K, int dtype, int epilogue, const void* residual, int64_t ld_res, void* stream);
 
 /*
+ * A Linear with 4-bit weights and group scales, activations as they come:
+ *   y[m, n] = sum_g scales[g, n] * sum_{k in g} x[m, k] * (code[n, k] - zeros[g, n]) + bias[n],   group g = inputs g * group and on,
+ * summed in fp32 and rounded to `dtype` once.  codes (N, K/2) contiguous, two to a byte, the even input in the lower half; scales
+ * (ceil(K / group), N) of type `dtype`, contiguous; zeros (ceil(K / group), N) uint8 or NULL, which stands for 8 throughout; bias fp32 (N)
+ * or NULL.  K % 8 == 0, group % 32 == 0 (the last group may be shorter); any N.  x has row stride ldx, a multiple of 8, and is 16-byte
+ * aligned, codes and bias are 4-byte aligned; y has row stride ldy, any.  `workspace`: samfast_linear_i4_workspace(M, N, K) bytes of device
+ * memory, 16-byte aligned, contents irrelevant before and after; NULL where that is 0.
+ * Over more than SAMFAST_I4_FEW_ROWS rows the weights (code - zero) * scale are rounded to `dtype` before they are
+ * multiplied: in fp16 they have to stay below 65504 there.
+ */
+#define SAMFAST_I4_FEW_ROWS 0
+int64_t samfast_linear_i4_workspace(int64_t M, int N, int K);
+int samfast_linear_i4(
+    const void* x, int64_t ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros, const float* bias,
+    void* y, int64_t ldy, void* workspace, int64_t M, int N, int K, int group, int dtype, void* stream);
+
+/*
+ * A block's end and the next one's beginning, row by row:
+ *   total = residual_scale * residual + branch_scale * gate * post(x),   normed = pre(total)
+ * with post and pre LayerNorms (or, with `rms`, RMS norms: v / sqrt(mean(v^2) + eps) * gamma + beta) over K <= 32768 values, each left
+ * out where its gamma is NULL (normed is then NULL too); a NULL beta is none.  x, gate, norm weights and normed are of type `dtype`, residual and
+ * total of it too or, with residual_is_f32, fp32.  gate: gate_rows rows of K, each for M / gate_rows rows, or NULL.  x and residual have row strides
+ * ldx and ld_res, the others are contiguous; any alignment.  fp32 throughout, pre of the total before it is
+ * rounded.  total may be the residual's memory (then ld_res == K).
+ */
+int samfast_norm_residual(
+    const void* x, int64_t ldx, const void* residual, int64_t ld_res, const void* gate, int64_t gate_rows,
+    const void* post_gamma, const void* post_beta, float post_eps,
+    const void* pre_gamma, const void* pre_beta, float pre_eps, int rms, float branch_scale, float residual_scale,
+    void* total, void* normed, int64_t M, int K, int dtype, int residual_is_f32, void* stream);
+
+/*
+ * Rotary positions in queries and keys: of the first 2 * axes * pairs of D channels, pair p of axis j, (a, b), becomes
+ *   (a cos t - b sin t, b cos t + a sin t) * magnitude,   t = positions[token, j] * frequencies[j, p],
+ * the others are copied.  An axis has 2 * pairs adjacent channels; its pairs are neighbours (`interleaved`) or a channel of the lower half and its
+ * like of the upper.  q and k are addressed as ptr + b*s_b + h*s_h + t*s_t + d; `strides` (host memory, read before the call returns): s_b, s_h, s_t of q,
+ * of q_out, of k, of k_out, in elements.  positions int64, axes a token, tokens contiguous, pos_sb between images (0: all the
+ * same); frequencies fp64 (axes, pairs).  The angle is made in fp64.  Any alignment.  q_out and k_out may be q and k.  With heads_k = 0 q alone.  D <= 1024.
+ */
+int samfast_rotary(
+    const void* q, const void* k, void* q_out, void* k_out, const int64_t* positions, int64_t pos_sb, const double* frequencies,
+    int64_t B, int64_t T, int heads_q, int heads_k, int D, int pairs, int axes, int interleaved, float magnitude,
+    const int64_t* strides, int dtype, void* stream);
+
+/*
  * A convolution of the neck (modeling/image_encoder.py:88-104) over channels-last half-type images: y (B, H, W, Cout) of x
  * (B, H, W, Cin), stride 1, no bias; taps = 1: 1 x 1, w (Cout, Cin); taps = 9: 3 x 3 with zero padding of one, w (Cout, 9, Cin).
  * With relay_src the launch also writes relay_dst (relay_rows, 9, relay_cin) from a 3 x 3 weight (relay_rows, relay_cin, 3, 3): the

@@ -41,6 +41,12 @@ _SIGNATURES = {
     "samfast_patch_rows": (_i32, [_ptr, _ptr, _i64, _i32, _i32, _i32, _ptr]),
     "samfast_linear_half_pays": (_i32, [_i64, _i32, _i32, _i32]),
     "samfast_linear_half": (_i32, [_ptr, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i32, _i32, _i32, _i32, _ptr, _i64, _ptr]),
+    "samfast_linear_i4_workspace": (_i64, [_i64, _i32, _i32]),
+    "samfast_linear_i4": (_i32, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _i32, _i32, _i32, _i32, _ptr]),
+    "samfast_norm_residual": (
+        _i32, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _f32, _ptr, _ptr, _f32, _i32, _f32, _f32, _ptr, _ptr, _i64, _i32, _i32, _i32, _ptr]),
+    "samfast_rotary": (
+        _i32, [_ptr] * 5 + [_i64, _ptr, _i64, _i64] + [_i32] * 6 + [_f32, ctypes.POINTER(_i64), _i32, _ptr]),
     "samfast_gelu_quant_rowwise_i8": (_i32, [_ptr, _i64, _ptr, _ptr, _i64, _i32, _i32, _i32, _ptr]),
     "samfast_linear_i8": (_i32, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _i32, _i32, _i32, _i32, _ptr]),
     "samfast_linear_i8_sparse24": (_i32, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _i32, _i32, _i32, _ptr]),

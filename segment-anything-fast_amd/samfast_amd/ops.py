@@ -670,6 +670,164 @@ def linear_half(x: torch.Tensor, linear: torch.nn.Linear, epilogue: int = _lib.E
     return out
 
 
+def _require_here(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Launches go to the current device's stream and leave no trace for a backward pass: tensors elsewhere, and ones that
+    autograd follows, are refused."""
+    _require_gpu(*tensors)
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device.index != device:
+            raise RuntimeError(f"samfast: {name} needs tensors on the current device, cuda:{device}, got one on {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"samfast: {name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
+def linear_i4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+              bias: Optional[torch.Tensor] = None, *, group_size: int) -> torch.Tensor:
+    """Linear with 4-bit weights on half-type rows x (..., K): y = x w^T + bias with w[n, k] = (code[n, k] - zeros[g, n]) * scales[g, n],
+    g = k // group_size.  codes: uint8 (N, K/2), the even k in the lower half of a byte; scales (groups, N) of x's dtype; zeros uint8 (groups, N),
+    or None for 8; bias fp32 (N).  K a multiple of 8, group_size of 32; the last group may be shorter.  Returns (..., N)."""
+    _require_here("linear_i4", x, codes, scales, zeros, bias)
+    dtype = _dtype_code(x)
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous():
+        raise RuntimeError("samfast: linear_i4 codes must be a contiguous uint8 (N, K/2) tensor")
+    N, K = codes.shape[0], 2 * codes.shape[1]
+    if N == 0 or K == 0 or K % 8 != 0 or group_size <= 0 or group_size % 32 != 0:
+        raise RuntimeError(f"samfast: linear_i4 needs K % 8 == 0 and groups of a multiple of 32 inputs, got K={K}, group_size={group_size}")
+    if x.dim() == 0 or x.shape[-1] != K:
+        raise RuntimeError(f"samfast: linear_i4 needs rows of {K} values, got {tuple(x.shape)}")
+    groups = -(-K // group_size)
+    if tuple(scales.shape) != (groups, N) or scales.dtype != x.dtype or not scales.is_contiguous():
+        raise RuntimeError(f"samfast: linear_i4 scales must be a contiguous ({groups}, {N}) tensor of x's dtype")
+    if zeros is not None and (tuple(zeros.shape) != (groups, N) or zeros.dtype != torch.uint8 or not zeros.is_contiguous()):
+        raise RuntimeError(f"samfast: linear_i4 zeros must be a contiguous uint8 ({groups}, {N}) tensor")
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
+        raise RuntimeError(f"samfast: linear_i4 bias must be fp32 of length {N}")
+    rows = x.reshape(-1, K)
+    if rows.stride(1) != 1 or rows.stride(0) % 8 != 0 or rows.stride(0) < K or rows.data_ptr() % 16 != 0:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+    M = rows.shape[0]
+    lib = _lib.load()
+    need = lib.samfast_linear_i4_workspace(M, N, K)
+    if need < 0:
+        _lib.check(int(need), "linear_i4_workspace")
+    work = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
+    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    code = _timed(
+        "linear_i4", 2.0 * M * N * K, "flop",
+        lambda: lib.samfast_linear_i4(
+            rows.data_ptr(), rows.stride(0), codes.data_ptr(), scales.data_ptr(), zeros.data_ptr() if zeros is not None else None,
+            bias.data_ptr() if bias is not None else None, y.data_ptr(), N, work.data_ptr() if work is not None else None,
+            M, N, K, group_size, dtype, _stream()))
+    _lib.check(code, "linear_i4")
+    return y
+
+
+def _norm_weights(name: str, norm, x: torch.Tensor):
+    """(gamma, beta, eps) of a norm given as (gamma, beta or None, eps), or of None."""
+    if norm is None:
+        return None, None, 0.0
+    gamma, beta, eps = norm
+    for t in (gamma, beta):
+        if t is not None and (t.dtype != x.dtype or tuple(t.shape) != (x.shape[-1],) or not t.is_contiguous()):
+            raise RuntimeError(f"samfast: the weights of {name} must be contiguous, of x's dtype and as long as its rows")
+    if gamma is None:
+        raise RuntimeError(f"samfast: {name} needs a weight")
+    return gamma, beta, float(eps)
+
+
+def norm_residual(x: torch.Tensor, residual: torch.Tensor, *, gate: Optional[torch.Tensor] = None, post=None, pre=None, rms: bool = False,
+                  branch_scale: float = 1.0, residual_scale: float = 1.0,
+                  out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """A block's end and the next one's beginning in one launch:
+        total = residual_scale * residual + branch_scale * gate * post(x),   normed = pre(total)
+    over the last axis of half-type rows x (..., K <= 32768).  post and pre: (gamma, beta or None, eps) of a LayerNorm, or with `rms` of an RMS
+    norm, or None to leave it out (normed is then None).  residual: x's shape, x's dtype or fp32; total has its type.  gate: (K), or (G, K) with a
+    row for each of G equal runs of x's rows.  fp32 inside; pre sees the total before it is rounded.  `out`: where total goes, which may be the
+    residual.  Returns (total, normed)."""
+    post_gamma, post_beta, post_eps = _norm_weights("post", post, x)
+    pre_gamma, pre_beta, pre_eps = _norm_weights("pre", pre, x)
+    _require_here("norm_residual", x, residual, gate, post_gamma, post_beta, pre_gamma, pre_beta, out)
+    dtype = _dtype_code(x)
+    if x.dim() == 0 or x.shape[-1] == 0 or residual.shape != x.shape or residual.dtype not in (x.dtype, torch.float32):
+        raise RuntimeError("samfast: norm_residual needs rows, and a residual of x's shape in x's dtype or fp32")
+    K = x.shape[-1]
+    M = x.numel() // K
+    gates = 1
+    if gate is not None:
+        if gate.dim() not in (1, 2) or gate.shape[-1] != K or gate.dtype != x.dtype or not gate.is_contiguous():
+            raise RuntimeError(f"samfast: norm_residual's gate must be a contiguous ({K},) or (groups, {K}) tensor of x's dtype")
+        gates = gate.shape[0] if gate.dim() == 2 else 1
+        if gates == 0 or M % gates != 0:
+            raise RuntimeError(f"samfast: {M} rows do not share {gates} gate rows evenly")
+    rows, res = x.reshape(M, K), residual.reshape(M, K)
+    if rows.stride(1) != 1 or rows.stride(0) < K:
+        rows = rows.contiguous()
+    if res.stride(1) != 1 or res.stride(0) < K:
+        res = res.contiguous()
+    if out is not None and (out.shape != x.shape or out.dtype != residual.dtype or not out.is_contiguous()):
+        raise RuntimeError("samfast: out must be a contiguous tensor of the residual's shape and dtype")
+    total = torch.empty(x.shape, dtype=residual.dtype, device=x.device) if out is None else out
+    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre is not None else None
+    ptr = lambda t: t.data_ptr() if t is not None else None
+    lib = _lib.load()
+    code = _timed(
+        "norm_residual", M * K * (2.0 + 2.0 * residual.element_size() + (2.0 if pre is not None else 0.0)), "byte",
+        lambda: lib.samfast_norm_residual(
+            rows.data_ptr(), rows.stride(0) if M > 1 else K, res.data_ptr(), res.stride(0) if M > 1 else K, ptr(gate), gates,
+            ptr(post_gamma), ptr(post_beta), post_eps, ptr(pre_gamma), ptr(pre_beta), pre_eps, int(rms),
+            float(branch_scale), float(residual_scale), total.data_ptr(), ptr(normed), M, K, dtype, int(residual.dtype == torch.float32), _stream()))
+    _lib.check(code, "norm_residual")
+    return total, normed
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor, *, interleaved: bool = False,
+           scale: float = 1.0, out: Optional[Tuple[torch.Tensor, Optional[torch.Tensor]]] = None):
+    """Rotary positions in queries and keys: q (B, nH, T, hd) and k (B, nKV, T, hd), any batch / head / token strides (head_dim contiguous), half
+    types.  positions int64, (B, T) or (T,); frequencies fp64 (pairs,), radians a position.  For a grid positions (..., T, axes) and
+    frequencies (axes, pairs).  Axis after axis, 2 * pairs channels of the head are turned: pairs of neighbours (`interleaved`), or of a channel
+    and its like half of the axis's channels on; channels behind the last axis's are copied.  `scale` multiplies what is turned.  Angles are made in 64
+    bits.  Returns (q', k') in q's and k's shapes, laid out token-major (k' is None where k is), or in `out`, which may be (q, k)."""
+    _require_here("rotary", q, k, positions, frequencies, *(out or ()))
+    dtype = _dtype_code(q)
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], *k.shape[2:]) != (q.shape[0], *q.shape[2:]))):
+        raise RuntimeError("samfast: rotary needs q (B, nH, T, hd) and k (B, nKV, T, hd) of one dtype")
+    B, H, T, D = q.shape
+    if frequencies.dtype != torch.float64 or frequencies.dim() not in (1, 2) or frequencies.numel() == 0 or not frequencies.is_contiguous():
+        raise RuntimeError("samfast: rotary frequencies must be a contiguous fp64 (pairs,) or (axes, pairs) tensor")
+    axes, pairs = (1, frequencies.shape[0]) if frequencies.dim() == 1 else tuple(frequencies.shape)
+    if 2 * axes * pairs > D:
+        raise RuntimeError(f"samfast: {axes} axes of {pairs} pairs do not fit into a head of {D} channels")
+    tail = () if frequencies.dim() == 1 else (axes,)
+    if positions.dtype != torch.int64 or tuple(positions.shape) not in ((B, T, *tail), (T, *tail)):
+        raise RuntimeError(f"samfast: rotary positions must be int64 of shape {(B, T, *tail)} or {(T, *tail)}")
+    shared = positions.dim() == 1 + len(tail)
+    positions = positions.contiguous()
+    tensors = [q] if k is None else [q, k]
+    if out is None:
+        outs = [torch.empty((B, T, t.shape[1], D), dtype=t.dtype, device=t.device).permute(0, 2, 1, 3) for t in tensors]
+    else:
+        outs = list(out[:len(tensors)])
+        for t, o in zip(tensors, outs):
+            if o is None or o.shape != t.shape or o.dtype != t.dtype:
+                raise RuntimeError("samfast: out must hold tensors of q's and k's shapes and dtype")
+    strides = []
+    for t, o in zip(tensors, outs):
+        strides += [*_bnhd_strides(t), *_bnhd_strides(o)]
+    strides += [0] * (12 - len(strides))
+    lib = _lib.load()
+    code = _timed(
+        "rotary", 4.0 * sum(t.numel() for t in tensors), "byte",
+        lambda: lib.samfast_rotary(
+            q.data_ptr(), k.data_ptr() if k is not None else None, outs[0].data_ptr(), outs[1].data_ptr() if k is not None else None,
+            positions.data_ptr(), 0 if shared else T * axes, frequencies.data_ptr(), B, T, H, k.shape[1] if k is not None else 0, D, pairs, axes,
+            int(interleaved), float(scale), (ctypes.c_int64 * 12)(*strides), dtype, _stream()))
+    _lib.check(code, "rotary")
+    return outs[0], outs[1] if k is not None else None
+
+
 def neck_convs(x: torch.Tensor, w1: torch.Tensor, norm, w3: torch.Tensor) -> torch.Tensor:
     """3x3 conv (w3, zero padding) of norm(1x1 conv (w1)) over contiguous channels-last half-type images (B, H, W, C);
     `norm` maps the (B, H, W, C1) rows in between.  Returns (B, H, W, C2)."""
