@@ -31,6 +31,10 @@ decltype(&samfast_linear_i8_workspace) p_linear_i8_workspace;
 decltype(&samfast_linear_i8_one_launch) p_linear_i8_one_launch;
 decltype(&samfast_linear_i8_sparse24) p_linear_i8_sparse24;
 decltype(&samfast_attn_relpos_bias_fwd) p_attn_bias;
+decltype(&samfast_linear_i4) p_linear_i4;
+decltype(&samfast_linear_i4_workspace) p_linear_i4_workspace;
+decltype(&samfast_norm_residual) p_norm_residual;
+decltype(&samfast_rotary) p_rotary;
 
 struct Bound { const char* name; void** slot; };
 const Bound kBound[] = {
@@ -39,6 +43,10 @@ const Bound kBound[] = {
     {"samfast_linear_i8_one_launch", reinterpret_cast<void**>(&p_linear_i8_one_launch)},
     {"samfast_linear_i8_sparse24", reinterpret_cast<void**>(&p_linear_i8_sparse24)},
     {"samfast_attn_relpos_bias_fwd", reinterpret_cast<void**>(&p_attn_bias)},
+    {"samfast_linear_i4", reinterpret_cast<void**>(&p_linear_i4)},
+    {"samfast_linear_i4_workspace", reinterpret_cast<void**>(&p_linear_i4_workspace)},
+    {"samfast_norm_residual", reinterpret_cast<void**>(&p_norm_residual)},
+    {"samfast_rotary", reinterpret_cast<void**>(&p_rotary)},
 };
 
 PyObject* device_context = nullptr;  // the mode of `with torch.device(..)` and torch.set_default_device, set by bind()
@@ -233,6 +241,147 @@ PyObject* host_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the operators without a backward pass: a tensor that autograd follows is the Python route's to refuse
+bool usable(const at::Tensor& t, c10::DeviceIndex dev) { return on_current_gpu(t, dev) && !(t.requires_grad() && c10::GradMode::is_enabled()); }
+bool is_half(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+int dtype_code(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? SAMFAST_F16 : SAMFAST_BF16; }
+// an argument that may be None: *t is then null; false for anything that is neither None nor a usable contiguous tensor of this type
+bool optional_arg(PyObject* o, c10::DeviceIndex dev, at::ScalarType type, const at::Tensor** t) {
+  *t = nullptr;
+  if (o == Py_None) return true;
+  *t = tensor_arg(o);
+  return *t && usable(**t, dev) && (*t)->scalar_type() == type && (*t)->is_contiguous();
+}
+const void* ptr_or_null(const at::Tensor* t) { return t ? ptr(*t) : nullptr; }
+
+// linear_i4(x, codes, scales, zeros or None, bias or None, group): the Linear with 4-bit weights on contiguous rows
+PyObject* host_linear_i4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !plain_call() || !PyLong_CheckExact(args[5])) Py_RETURN_NONE;
+  const at::Tensor *x = tensor_arg(args[0]), *codes = tensor_arg(args[1]), *scales = tensor_arg(args[2]), *zeros, *bias;
+  if (!x || !codes || !scales || !x->is_cuda()) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  int overflow = 0;
+  const int64_t group = PyLong_AsLongLongAndOverflow(args[5], &overflow);
+  if (overflow || group <= 0 || group > INT32_MAX) Py_RETURN_NONE;
+  for (const at::Tensor* t : {x, codes, scales})
+    if (!usable(*t, dev) || !t->is_contiguous()) Py_RETURN_NONE;
+  if (!is_half(*x) || x->dim() < 1 || x->numel() == 0 || codes->dim() != 2 || codes->scalar_type() != at::kByte || scales->scalar_type() != x->scalar_type())
+    Py_RETURN_NONE;
+  const int64_t N = codes->size(0), K = 2 * codes->size(1);
+  if (N <= 0 || N > INT32_MAX || K <= 0 || K > INT32_MAX || x->size(-1) != K) Py_RETURN_NONE;
+  if (!optional_arg(args[3], dev, at::kByte, &zeros) || !optional_arg(args[4], dev, at::kFloat, &bias)) Py_RETURN_NONE;
+  const int64_t groups = (K + group - 1) / group, M = x->numel() / K;
+  if (scales->dim() != 2 || scales->size(0) != groups || scales->size(1) != N || (zeros && zeros->sizes() != scales->sizes()) ||
+      (bias && (bias->dim() != 1 || bias->size(0) != N)))
+    Py_RETURN_NONE;
+  const int64_t need = p_linear_i4_workspace(M, static_cast<int>(N), static_cast<int>(K));
+  if (need < 0) Py_RETURN_NONE;
+  at::Tensor work;
+  if (need > 0) work = new_tensor({need}, at::kByte, dev);
+  c10::SmallVector<int64_t, 5> shape(x->sizes().begin(), x->sizes().end());
+  shape.back() = N;
+  at::Tensor y = new_tensor(shape, x->scalar_type(), dev);
+  const int rc = p_linear_i4(ptr(*x), K, static_cast<const uint8_t*>(ptr(*codes)), ptr(*scales), static_cast<const uint8_t*>(ptr_or_null(zeros)),
+                             static_cast<const float*>(ptr_or_null(bias)), y.data_ptr(), N, need > 0 ? work.data_ptr() : nullptr, M,
+                             static_cast<int>(N), static_cast<int>(K), static_cast<int>(group), dtype_code(*x), stream_of(dev));
+  if (rc != SAMFAST_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// a norm as (gamma, beta or None, eps), or None
+struct NormArg {
+  const at::Tensor *gamma = nullptr, *beta = nullptr;
+  float eps = 0.f;
+  bool read(PyObject* o, c10::DeviceIndex dev, at::ScalarType type, int64_t K) {
+    if (o == Py_None) return true;
+    if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 3 || !PyFloat_CheckExact(PyTuple_GET_ITEM(o, 2))) return false;
+    eps = static_cast<float>(PyFloat_AS_DOUBLE(PyTuple_GET_ITEM(o, 2)));
+    if (!optional_arg(PyTuple_GET_ITEM(o, 0), dev, type, &gamma) || !optional_arg(PyTuple_GET_ITEM(o, 1), dev, type, &beta)) return false;
+    return gamma && gamma->dim() == 1 && gamma->size(0) == K && (!beta || (beta->dim() == 1 && beta->size(0) == K));
+  }
+};
+
+// norm_residual(x, residual, gate or None, post or None, pre or None, rms, branch_scale, residual_scale) on contiguous rows: (total, normed or None)
+PyObject* host_norm_residual(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || !plain_call() || !PyBool_Check(args[5]) || !PyFloat_CheckExact(args[6]) || !PyFloat_CheckExact(args[7])) Py_RETURN_NONE;
+  const at::Tensor *x = tensor_arg(args[0]), *residual = tensor_arg(args[1]), *gate;
+  if (!x || !residual || !x->is_cuda()) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  for (const at::Tensor* t : {x, residual})
+    if (!usable(*t, dev) || !t->is_contiguous()) Py_RETURN_NONE;
+  if (!is_half(*x) || x->dim() < 1 || x->numel() == 0 || residual->sizes() != x->sizes() ||
+      (residual->scalar_type() != x->scalar_type() && residual->scalar_type() != at::kFloat))
+    Py_RETURN_NONE;
+  const int64_t K = x->size(-1), M = x->numel() / K;
+  NormArg post, pre;
+  if (K > INT32_MAX || !optional_arg(args[2], dev, x->scalar_type(), &gate) || !post.read(args[3], dev, x->scalar_type(), K) || !pre.read(args[4], dev, x->scalar_type(), K))
+    Py_RETURN_NONE;
+  int64_t gates = 1;
+  if (gate) {
+    if (gate->dim() < 1 || gate->dim() > 2 || gate->size(-1) != K) Py_RETURN_NONE;
+    gates = gate->dim() == 2 ? gate->size(0) : 1;
+    if (gates == 0) Py_RETURN_NONE;  // (no memory: it would pass for no gate)
+  }
+  at::Tensor total = new_tensor(x->sizes(), residual->scalar_type(), dev), normed;
+  if (pre.gamma) normed = new_tensor(x->sizes(), x->scalar_type(), dev);
+  const int rc = p_norm_residual(ptr(*x), K, ptr(*residual), K, ptr_or_null(gate), gates, ptr_or_null(post.gamma), ptr_or_null(post.beta), post.eps,
+                                 ptr_or_null(pre.gamma), ptr_or_null(pre.beta), pre.eps, args[5] == Py_True,
+                                 static_cast<float>(PyFloat_AS_DOUBLE(args[6])), static_cast<float>(PyFloat_AS_DOUBLE(args[7])), total.data_ptr(),
+                                 pre.gamma ? normed.data_ptr() : nullptr, M, static_cast<int>(K), dtype_code(*x), residual->scalar_type() == at::kFloat,
+                                 stream_of(dev));
+  if (rc != SAMFAST_OK) Py_RETURN_NONE;
+  PyObject* first = THPVariable_Wrap(std::move(total));
+  PyObject* second = pre.gamma ? THPVariable_Wrap(std::move(normed)) : Py_NewRef(Py_None);
+  return Py_BuildValue("(NN)", first, second);
+  END_HANDLE_TH_ERRORS
+}
+
+// rotary(q, k or None, positions, frequencies, interleaved, scale): (q', k' or None), token-major
+PyObject* host_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !plain_call() || !PyBool_Check(args[4]) || !PyFloat_CheckExact(args[5])) Py_RETURN_NONE;
+  const at::Tensor *q = tensor_arg(args[0]), *k = nullptr, *pos = tensor_arg(args[2]), *freq = tensor_arg(args[3]);
+  if (args[1] != Py_None && !(k = tensor_arg(args[1]))) Py_RETURN_NONE;
+  if (!q || !pos || !freq || !q->is_cuda()) Py_RETURN_NONE;
+  const c10::DeviceIndex dev = c10::hip::current_device();
+  for (const at::Tensor* t : {q, pos, freq})
+    if (!usable(*t, dev)) Py_RETURN_NONE;
+  if (!is_half(*q) || q->dim() != 4 || q->numel() == 0 || q->stride(3) != 1 || pos->scalar_type() != at::kLong || !pos->is_contiguous() ||
+      freq->scalar_type() != at::kDouble || !freq->is_contiguous() || freq->numel() == 0 || freq->dim() < 1 || freq->dim() > 2)
+    Py_RETURN_NONE;
+  const int64_t B = q->size(0), H = q->size(1), T = q->size(2), D = q->size(3), KV = k ? k->size(1) : 0;
+  if (k && (!usable(*k, dev) || k->scalar_type() != q->scalar_type() || k->dim() != 4 || k->size(0) != B || k->size(2) != T || k->size(3) != D || k->stride(3) != 1))
+    Py_RETURN_NONE;
+  const bool grid = freq->dim() == 2;
+  const int64_t axes = grid ? freq->size(0) : 1, pairs = freq->size(-1);
+  const int64_t lead = pos->dim() - (grid ? 1 : 0);  // 1: the same positions in every image
+  if (axes > INT32_MAX || pairs > INT32_MAX || D > INT32_MAX || H > INT32_MAX || KV > INT32_MAX || lead < 1 || lead > 2 || (lead == 2 && pos->size(0) != B) ||
+      pos->size(lead - 1) != T || (grid && pos->size(lead) != axes))
+    Py_RETURN_NONE;
+  const auto like = [&](int64_t heads) {
+    return at::detail::empty_strided_cuda({B, heads, T, D}, {T * heads * D, D, heads * D, 1}, q->scalar_type(), c10::Device(c10::kCUDA, dev));
+  };
+  at::Tensor q_out = like(H), k_out;
+  if (k) k_out = like(KV);
+  int64_t strides[12] = {q->stride(0), q->stride(1), q->stride(2), T * H * D, D, H * D};
+  if (k) {
+    const int64_t of_k[6] = {k->stride(0), k->stride(1), k->stride(2), T * KV * D, D, KV * D};
+    for (int i = 0; i < 6; ++i) strides[6 + i] = of_k[i];
+  }
+  const int rc = p_rotary(ptr(*q), ptr_or_null(k), q_out.data_ptr(), k ? k_out.data_ptr() : nullptr, static_cast<const int64_t*>(ptr(*pos)),
+                          lead == 1 ? 0 : T * axes, static_cast<const double*>(ptr(*freq)), B, T, static_cast<int>(H), static_cast<int>(KV),
+                          static_cast<int>(D), static_cast<int>(pairs), static_cast<int>(axes), args[4] == Py_True,
+                          static_cast<float>(PyFloat_AS_DOUBLE(args[5])), strides, dtype_code(*q), stream_of(dev));
+  if (rc != SAMFAST_OK) Py_RETURN_NONE;
+  PyObject* first = THPVariable_Wrap(std::move(q_out));
+  PyObject* second = k ? THPVariable_Wrap(std::move(k_out)) : Py_NewRef(Py_None);
+  return Py_BuildValue("(NN)", first, second);
+  END_HANDLE_TH_ERRORS
+}
+
 // plain(tensor): whether a launch that only the kernels see may stand for operations on this tensor
 PyObject* host_plain(PyObject*, PyObject* arg) {
   const at::Tensor* t = tensor_arg(arg);
@@ -280,6 +429,9 @@ PyMethodDef kMethods[] = {
     {"module_linear", fastcall(host_module_linear), METH_FASTCALL, nullptr},
     {"module_sparse_linear", fastcall(host_module_sparse_linear), METH_FASTCALL, nullptr},
     {"attention", fastcall(host_attention), METH_FASTCALL, nullptr},
+    {"linear_i4", fastcall(host_linear_i4), METH_FASTCALL, nullptr},
+    {"norm_residual", fastcall(host_norm_residual), METH_FASTCALL, nullptr},
+    {"rotary", fastcall(host_rotary), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_samfast_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -689,6 +689,10 @@ def linear_i4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     """Linear with 4-bit weights on half-type rows x (..., K): y = x w^T + bias with w[n, k] = (code[n, k] - zeros[g, n]) * scales[g, n],
     g = k // group_size.  codes: uint8 (N, K/2), the even k in the lower half of a byte; scales (groups, N) of x's dtype; zeros uint8 (groups, N),
     or None for 8; bias fp32 (N).  K a multiple of 8, group_size of 32; the last group may be shorter.  Returns (..., N)."""
+    if _launch_log is None:
+        y = (_lib._host or _lib.host()).linear_i4(x, codes, scales, zeros, bias, group_size)
+        if y is not None:
+            return y
     _require_here("linear_i4", x, codes, scales, zeros, bias)
     dtype = _dtype_code(x)
     if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous():
@@ -747,6 +751,10 @@ def norm_residual(x: torch.Tensor, residual: torch.Tensor, *, gate: Optional[tor
     norm, or None to leave it out (normed is then None).  residual: x's shape, x's dtype or fp32; total has its type.  gate: (K), or (G, K) with a
     row for each of G equal runs of x's rows.  fp32 inside; pre sees the total before it is rounded.  `out`: where total goes, which may be the
     residual.  Returns (total, normed)."""
+    if out is None and _launch_log is None:
+        both = (_lib._host or _lib.host()).norm_residual(x, residual, gate, post, pre, rms, branch_scale, residual_scale)
+        if both is not None:
+            return both
     post_gamma, post_beta, post_eps = _norm_weights("post", post, x)
     pre_gamma, pre_beta, pre_eps = _norm_weights("pre", pre, x)
     _require_here("norm_residual", x, residual, gate, post_gamma, post_beta, pre_gamma, pre_beta, out)
@@ -790,6 +798,10 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     frequencies (axes, pairs).  Axis after axis, 2 * pairs channels of the head are turned: pairs of neighbours (`interleaved`), or of a channel
     and its like half of the axis's channels on; channels behind the last axis's are copied.  `scale` multiplies what is turned.  Angles are made in 64
     bits.  Returns (q', k') in q's and k's shapes, laid out token-major (k' is None where k is), or in `out`, which may be (q, k)."""
+    if out is None and _launch_log is None:
+        both = (_lib._host or _lib.host()).rotary(q, k, positions, frequencies, interleaved, scale)
+        if both is not None:
+            return both
     _require_here("rotary", q, k, positions, frequencies, *(out or ()))
     dtype = _dtype_code(q)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], *k.shape[2:]) != (q.shape[0], *q.shape[2:]))):
