@@ -48,7 +48,7 @@ struct PPArgs {
   unsigned short* out;
   const float* sx;         // int8: row scales, column scales
   const float* sw;
-  const void* bias;        // int8: fp32, else the element type; may be null
+  const void* bias;        // int8 and BIAS32: fp32, else the element type; may be null
   const unsigned short* residual;
   int64_t ldo, ld_res;     // elements
   int64_t x_kstep, w_kstep;
@@ -60,13 +60,13 @@ struct PPArgs {
 struct PPInt8 {
   typedef i32x4 acc_t;
   typedef ElemBf16 Out;
-  static constexpr bool SCALED = true;
+  static constexpr bool SCALED = true, BIAS32 = false;
   static SF_DEVICE acc_t mma(i32x4 a, i32x4 b, acc_t c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 };
 struct PPBf16 {
   typedef f32x4 acc_t;
   typedef ElemBf16 Out;
-  static constexpr bool SCALED = false;
+  static constexpr bool SCALED = false, BIAS32 = false;
   static SF_DEVICE acc_t mma(i32x4 a, i32x4 b, acc_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -74,11 +74,19 @@ struct PPBf16 {
 struct PPF16 {
   typedef f32x4 acc_t;
   typedef ElemF16 Out;
-  static constexpr bool SCALED = false;
+  static constexpr bool SCALED = false, BIAS32 = false;
   typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
   static SF_DEVICE acc_t mma(i32x4 a, i32x4 b, acc_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
   }
+};
+
+// half types with an fp32 bias (the resident kernel)
+struct PPBf16Bias32 : PPBf16 {
+  static constexpr bool BIAS32 = true;
+};
+struct PPF16Bias32 : PPF16 {
+  static constexpr bool BIAS32 = true;
 };
 
 enum { PP_PLAIN = 0, PP_GELU = 1, PP_RESIDUAL = 2 };
@@ -230,6 +238,9 @@ __global__ __launch_bounds__(512, 2) void gemm_pingpong_kernel(PPArgs a) {
         const int dst = (part == 0 ? 0 : part == 1 ? P::BM * 4 : P::BM * 4 + P::BN * 4) + q * 4;
         __builtin_amdgcn_global_load_lds((gptr_t)(src + q + lane), (lptr_t)(sc + dst), 4, 0, 0);
       }
+    } else if constexpr (E::BIAS32) {
+      const int q = wave % (P::BN / 64) * 64;
+      if (a.bias) __builtin_amdgcn_global_load_lds((gptr_t)(reinterpret_cast<const float*>(a.bias) + n0 + q + lane), (lptr_t)(sc + q * 4), 4, 0, 0);
     } else {
       // columns in pairs (N is even); 320 columns are two and a half slices, 192 one and a half: they overlap
       const int q = P::BN == 320 ? (wave % 3) * 96 : (wave & 1) * (P::BN - 128);
@@ -352,6 +363,8 @@ __global__ __launch_bounds__(512, 2) void gemm_pingpong_kernel(PPArgs a) {
         if constexpr (E::SCALED) {
           sw[g][e] = reinterpret_cast<const float*>(sc + P::BM * 4 + col * 4)[e];
           bias[g][e] = a.bias ? reinterpret_cast<const float*>(sc + P::BM * 4 + P::BN * 4 + col * 4)[e] : 0.f;
+        } else if constexpr (E::BIAS32) {
+          bias[g][e] = a.bias ? reinterpret_cast<const float*>(sc + col * 4)[e] : 0.f;
         } else {
           const unsigned int b = a.bias ? reinterpret_cast<const unsigned int*>(sc + col * 2)[e >> 1] : 0u;
           bias[g][e] = e & 1 ? Out::hi(b) : Out::lo(b);

@@ -177,7 +177,7 @@ static int launch_i4_tiled(I4Args a, hipStream_t stream) {
 extern "C" int64_t samfast_linear_i4_workspace(int64_t M, int N, int K) {
   using namespace samfast;
   SF_REQUIRE(M >= 0 && N > 0 && K > 0, "linear_i4_workspace: bad shape M=%lld N=%d K=%d", (long long)M, N, K);
-  return 0;
+  return i4_dense_tile(M, N, K) ? (int64_t)N * K * 2 : 0;
 }
 
 extern "C" int samfast_linear_i4(const void* x, int64_t ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros, const float* bias,
@@ -207,5 +207,9 @@ extern "C" int samfast_linear_i4(const void* x, int64_t ldx, const uint8_t* code
   a.K = K;
   a.group = group;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int tile = i4_dense_tile(M, N, K);
+  SF_REQUIRE(tile == 0 || (workspace && aligned16(workspace)), "linear_i4: this shape needs a 16-byte aligned workspace (samfast_linear_i4_workspace)");
+  if (tile != 0 && ldy % 8 == 0 && ldy < (1 << 22) && aligned16(y)) return launch_i4_dense(a, dtype == SAMFAST_F16, tile, workspace, s);
+  if (M <= SAMFAST_I4_FEW_ROWS) return launch_i4_few(a, dtype == SAMFAST_F16, s);
   return dtype == SAMFAST_F16 ? launch_i4_tiled<ElemF16>(a, s) : launch_i4_tiled<ElemBf16>(a, s);
 }

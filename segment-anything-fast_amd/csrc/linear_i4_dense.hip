@@ -1,0 +1,63 @@
+// Linears with 4-bit weights over many rows where the half types' product by turns (gemm_pingpong.hpp) fits: the weights are written out in the
+// element type, once per call, and that product reads them out of the caches.
+#include "gemm_pingpong.hpp"
+#include "linear_i4_shared.hpp"
+
+namespace samfast {
+
+// w[n, k] = (code - zero) * scale, rounded to the element type: eight codes a thread
+template <class T>
+__global__ __launch_bounds__(256) void i4_weights_kernel(I4Args a, unsigned short* w) {
+  const unsigned int words = (unsigned int)a.K / 8u;  // of a row
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.N * words) return;
+  const int n = (int)(i / words), k = 8 * (int)(i - (int64_t)n * words);
+  const int64_t at = (int64_t)(k / a.group) * a.N + n;
+  const float s = T::from_bits(a.scales[at]), z = a.zeros ? (float)a.zeros[at] : 8.f;
+  float c[8];
+  i4_codes(reinterpret_cast<const unsigned int*>(a.codes)[i], c);
+  u32x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = T::pack2((c[2 * e] - z) * s, (c[2 * e + 1] - z) * s);
+  reinterpret_cast<u32x4*>(w)[i] = o;
+}
+
+int i4_dense_tile(int64_t M, int N, int K) {
+  if (K % 64 != 0 || K < 320 || N % 8 != 0 || M < 512) return 0;
+  const PPChoice c = pp_choose(M, N, K / 64, false, 8.1);
+  return c.tn != 0 && c.used >= 0.5 ? c.tn : 0;
+}
+
+template <class T, class E>
+static int go_dense(const I4Args& a, int tile, unsigned short* weights, hipStream_t stream) {
+  const int64_t words = (int64_t)a.N * (a.K / 8);
+  hipLaunchKernelGGL(i4_weights_kernel<T>, dim3((unsigned int)((words + 255) / 256)), dim3(256), 0, stream, a, weights);
+  if (const int rc = check_launch("i4_weights_kernel")) return rc;
+  PPArgs p = {};
+  p.x = reinterpret_cast<const unsigned char*>(a.x);
+  p.w = reinterpret_cast<const unsigned char*>(weights);
+  p.out = a.y;
+  p.bias = a.bias;
+  p.ldo = a.ldy;
+  p.x_kstep = p.w_kstep = 64;
+  p.x_pitch = (unsigned int)(a.ldx * 2);
+  p.w_pitch = (unsigned int)(a.K * 2);
+  p.M = a.M;
+  p.N = a.N;
+  p.nk = a.K / 64;
+  p.group_m = 4;
+  p.tiles_m = (a.M + 255) / 256;
+  p.tiles_n = (a.N + 32 * tile - 1) / (32 * tile);
+  const dim3 grid(pp_grid(p));
+  if (tile == 6) hipLaunchKernelGGL((gemm_pingpong_kernel<E, PP_PLAIN, 6, false>), grid, dim3(512), 0, stream, p);
+  else if (tile == 8) hipLaunchKernelGGL((gemm_pingpong_kernel<E, PP_PLAIN, 8, false>), grid, dim3(512), 0, stream, p);
+  else hipLaunchKernelGGL((gemm_pingpong_kernel<E, PP_PLAIN, 10, false>), grid, dim3(512), 0, stream, p);
+  return check_launch("gemm_pingpong_kernel");
+}
+
+int launch_i4_dense(const I4Args& a, bool f16, int tile, void* weights, hipStream_t stream) {
+  unsigned short* w = reinterpret_cast<unsigned short*>(weights);
+  return f16 ? go_dense<ElemF16, PPF16Bias32>(a, tile, w, stream) : go_dense<ElemBf16, PPBf16Bias32>(a, tile, w, stream);
+}
+
+}  // namespace samfast
