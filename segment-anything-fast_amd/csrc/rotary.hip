@@ -8,6 +8,8 @@
 #include "samfast_internal.hpp"
 #include "attn_relpos_shared.hpp"
 
+#include <type_traits>
+
 namespace samfast {
 
 struct RotarySide {
@@ -22,10 +24,10 @@ struct RotaryArgs {
   int64_t pos_b;
   float magnitude;
   int tokens, T, heads_q, heads, D, pairs, axes;
-  int items, copies_at;       // pieces of a head, and the first of those that are only copied
+  int items;                  // pieces of a head
+  int chunks, copies;         // halves: pieces of an axis, pieces that are only copied
   int block_tokens, block_heads;
-  unsigned int div_items, div_heads, div_chunks;  // 2^32 / d, rounded up: x / d is the upper half of a product where x d < 2^32
-  int chunks;                 // halves: pieces of an axis
+  unsigned int div_items, div_turned, div_copies, div_heads, div_chunks;  // 2^32 / d, rounded up: x / d is the upper half of a product where x d < 2^32
 };
 
 constexpr int kRotaryThreads = 256;
@@ -33,6 +35,7 @@ constexpr int kRotaryPiece = 8;       // channels (halves: pairs) of a piece
 constexpr int kRotaryItems = 2048;    // pieces of a workgroup, unless one head has more
 constexpr int kRotaryTable = 1024;    // angles of a workgroup
 constexpr int kRotaryMaxDim = 1024;
+enum { kNeighbours, kHalves, kCopies };
 
 SF_DEVICE u32x4 load_any(const unsigned short* p) {  // 16 bytes from any even address
   u32x4 v;
@@ -77,63 +80,99 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   const int h0 = blockIdx.y * a.block_heads, nh = min(a.block_heads, a.heads - h0);
   const int angles = a.axes * a.pairs;
 
-  for (int i = threadIdx.x; i < nt * angles; i += kRotaryThreads) {
-    const int t = i / angles, p = i - t * angles;
-    int64_t b, n;
-    place(t, b, n);
-    const double pos = (double)a.pos[b * a.pos_b + n * a.axes + (a.axes == 1 ? 0 : p / a.pairs)];
-    double turns = pos * (a.freq[p] * 0.15915494309189535);  // 1 / 2 pi
-    turns -= rint(turns);
-    float s, c;
-    sincospif(2.0f * (float)turns, &s, &c);
-    table[i] = f32x2{c * a.magnitude, s * a.magnitude};
-  }
-  __syncthreads();
-
-  const unsigned int total = (unsigned int)(nt * nh * a.items);
-  for (unsigned int i = threadIdx.x; i < total; i += kRotaryThreads) {
-    const unsigned int row = a.items == 1 ? i : __umulhi(i, a.div_items);
-    const int item = (int)(i - row * a.items);
-    const int t = a.block_heads == 1 ? (int)row : (int)__umulhi(row, a.div_heads);  // (0 where heads are split: one token then)
-    int h = h0 + (int)row - t * nh;
-    int64_t b, token;
-    place(t, b, token);
-    const RotarySide& s = a.side[h >= a.heads_q];
-    if (h >= a.heads_q) h -= a.heads_q;
-    const unsigned short* in = s.in + b * s.in_b + h * s.in_h + token * s.in_t;
-    unsigned short* out = s.out + b * s.out_b + h * s.out_h + token * s.out_t;
-    const f32x2* cs = table + t * angles;
-    if (INTERLEAVED) {
-      const int d = item * kRotaryPiece, n = min(kRotaryPiece, a.D - d);
-      const u32x4 v = load_some(in + d, n);
-      u32x4 o;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool turned = d / 2 + j < angles;
-        const f32x2 w = cs[turned ? d / 2 + j : 0];
-        const float x = T::lo(v[j]), y = T::hi(v[j]);
-        o[j] = turned ? T::pack2(x * w[0] - y * w[1], y * w[0] + x * w[1]) : v[j];
-      }
-      store_some(out + d, o, n);
-    } else if (item < a.copies_at) {
-      const int axis = a.axes == 1 ? 0 : a.chunks == 1 ? item : (int)__umulhi((unsigned int)item, a.div_chunks);
-      const int p = (item - axis * a.chunks) * kRotaryPiece, n = min(kRotaryPiece, a.pairs - p);
-      const int d = 2 * axis * a.pairs + p;
-      const u32x4 x = load_some(in + d, n), y = load_some(in + d + a.pairs, n);
-      u32x4 ox, oy;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x2 w0 = cs[axis * a.pairs + min(p + 2 * j, a.pairs - 1)], w1 = cs[axis * a.pairs + min(p + 2 * j + 1, a.pairs - 1)];
-        const float x0 = T::lo(x[j]), x1 = T::hi(x[j]), y0 = T::lo(y[j]), y1 = T::hi(y[j]);
-        ox[j] = T::pack2(x0 * w0[0] - y0 * w0[1], x1 * w1[0] - y1 * w1[1]);
-        oy[j] = T::pack2(y0 * w0[0] + x0 * w0[1], y1 * w1[0] + x1 * w1[1]);
-      }
-      store_some(out + d, ox, n);
-      store_some(out + d + a.pairs, oy, n);
-    } else {
-      const int d = 2 * angles + (item - a.copies_at) * kRotaryPiece, n = min(kRotaryPiece, a.D - d);
-      store_some(out + d, load_some(in + d, n), n);
+  auto make_table = [&]() __attribute__((always_inline)) {
+    for (int i = threadIdx.x; i < nt * angles; i += kRotaryThreads) {
+      const int t = i / angles, p = i - t * angles;
+      int64_t b, n;
+      place(t, b, n);
+      const double pos = (double)a.pos[b * a.pos_b + n * a.axes + (a.axes == 1 ? 0 : p / a.pairs)];
+      double turns = pos * (a.freq[p] * 0.15915494309189535);  // 1 / 2 pi
+      turns -= rint(turns);
+      float s, c;
+      sincospif(2.0f * (float)turns, &s, &c);
+      table[i] = f32x2{c * a.magnitude, s * a.magnitude};
     }
+    __syncthreads();
+  };
+
+  // The pieces of one kind, `items` of them to a head, UNROLL of a thread at a time with all their loads in flight; before the first are used,
+  // `ready` is called.
+  auto walk = [&](auto kind, unsigned int items, unsigned int div, auto ready) __attribute__((always_inline)) {
+    constexpr int KIND = decltype(kind)::value;
+    constexpr int UNROLL = KIND == kHalves ? 2 : 4;
+    const unsigned int total = (unsigned int)(nt * nh) * items;
+    bool first_round = true;
+    for (unsigned int i0 = threadIdx.x; first_round || i0 < total; i0 += UNROLL * kRotaryThreads) {
+      u32x4 x[UNROLL], y[UNROLL];
+      unsigned short* out[UNROLL];
+      int at[UNROLL], n[UNROLL], turned[UNROLL];  // first angle, channels (halves: pairs), neighbours: pairs from here on that are turned
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const unsigned int i = i0 + u * kRotaryThreads;
+        n[u] = 0;
+        if (i >= total) continue;
+        const unsigned int row = items == 1 ? i : __umulhi(i, div);
+        const int item = (int)(i - row * items);
+        const int t = a.block_heads == 1 ? (int)row : (int)__umulhi(row, a.div_heads);  // (0 where heads are split: one token then)
+        int h = h0 + (int)row - t * nh;
+        int64_t b, token;
+        place(t, b, token);
+        const RotarySide& s = a.side[h >= a.heads_q];
+        if (h >= a.heads_q) h -= a.heads_q;
+        int d = item * kRotaryPiece;
+        at[u] = t * angles + d / 2;
+        turned[u] = angles - d / 2;
+        if (KIND == kHalves) {
+          const int axis = a.axes == 1 ? 0 : a.chunks == 1 ? item : (int)__umulhi((unsigned int)item, a.div_chunks);
+          const int p = d - axis * a.chunks * kRotaryPiece;
+          n[u] = min(kRotaryPiece, a.pairs - p);
+          at[u] = t * angles + axis * a.pairs + p;
+          d = 2 * axis * a.pairs + p;
+        } else {
+          if (KIND == kCopies) d += 2 * angles;
+          n[u] = min(kRotaryPiece, a.D - d);
+        }
+        const unsigned short* in = s.in + b * s.in_b + h * s.in_h + token * s.in_t + d;
+        out[u] = s.out + b * s.out_b + h * s.out_h + token * s.out_t + d;
+        x[u] = load_some(in, n[u]);
+        if (KIND == kHalves) y[u] = load_some(in + a.pairs, n[u]);
+      }
+      if (first_round) ready();
+      first_round = false;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        if (n[u] == 0) continue;
+        if (KIND == kNeighbours) {
+          u32x4 o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x2 w = table[j < turned[u] ? at[u] + j : 0];
+            const float v0 = T::lo(x[u][j]), v1 = T::hi(x[u][j]);
+            o[j] = j < turned[u] ? T::pack2(v0 * w[0] - v1 * w[1], v1 * w[0] + v0 * w[1]) : x[u][j];
+          }
+          store_some(out[u], o, n[u]);
+        } else if (KIND == kHalves) {
+          u32x4 ox, oy;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x2 w0 = table[at[u] + min(2 * j, n[u] - 1)], w1 = table[at[u] + min(2 * j + 1, n[u] - 1)];
+            const float x0 = T::lo(x[u][j]), x1 = T::hi(x[u][j]), y0 = T::lo(y[u][j]), y1 = T::hi(y[u][j]);
+            ox[j] = T::pack2(x0 * w0[0] - y0 * w0[1], x1 * w1[0] - y1 * w1[1]);
+            oy[j] = T::pack2(y0 * w0[0] + x0 * w0[1], y1 * w1[0] + x1 * w1[1]);
+          }
+          store_some(out[u], ox, n[u]);
+          store_some(out[u] + a.pairs, oy, n[u]);
+        } else {
+          store_some(out[u], x[u], n[u]);
+        }
+      }
+    }
+  };
+  if (INTERLEAVED) {
+    walk(std::integral_constant<int, kNeighbours>{}, (unsigned int)a.items, a.div_items, make_table);
+  } else {
+    walk(std::integral_constant<int, kHalves>{}, (unsigned int)(a.axes * a.chunks), a.div_turned, make_table);
+    if (a.copies > 0) walk(std::integral_constant<int, kCopies>{}, (unsigned int)a.copies, a.div_copies, [] {});
   }
 }
 
@@ -182,8 +221,8 @@ extern "C" int samfast_rotary(const void* q, const void* k, void* q_out, void* k
   a.axes = axes;
   const int angles = axes * pairs;
   a.chunks = (pairs + kRotaryPiece - 1) / kRotaryPiece;
-  a.copies_at = interleaved ? 0 : axes * a.chunks;
-  a.items = interleaved ? (D + kRotaryPiece - 1) / kRotaryPiece : a.copies_at + (D - 2 * angles + kRotaryPiece - 1) / kRotaryPiece;
+  a.copies = (D - 2 * angles + kRotaryPiece - 1) / kRotaryPiece;
+  a.items = interleaved ? (D + kRotaryPiece - 1) / kRotaryPiece : axes * a.chunks + a.copies;
   // a workgroup's share: kRotaryItems pieces, fewer where that leaves CUs without one
   int64_t share = (int64_t)a.tokens * a.heads * a.items / 1024;
   share = share < kRotaryThreads ? kRotaryThreads : share > kRotaryItems ? kRotaryItems : share;
@@ -196,6 +235,8 @@ extern "C" int samfast_rotary(const void* q, const void* k, void* q_out, void* k
   a.block_tokens = (int)(tokens < 1 ? 1 : tokens);
   SF_REQUIRE(parts < 65536, "rotary: too many heads");
   a.div_items = a.items > 1 ? divider(a.items) : 0;
+  a.div_turned = axes * a.chunks > 1 ? divider(axes * a.chunks) : 0;
+  a.div_copies = a.copies > 1 ? divider(a.copies) : 0;
   a.div_heads = a.block_heads > 1 ? divider(a.block_heads) : 0;
   a.div_chunks = a.chunks > 1 ? divider(a.chunks) : 0;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
