@@ -8,6 +8,8 @@
 #include "quant_row.hpp"
 #include "attn_relpos_shared.hpp"
 
+#include <type_traits>
+
 namespace samfast {
 
 struct NormResidualArgs {
@@ -18,8 +20,8 @@ struct NormResidualArgs {
   void* total;
   unsigned short* normed;    // null: no pre norm
   int64_t M, ldx, ld_res, group;  // rows that share a gate row
-  int64_t run;               // rows of a row's threads
   int K;
+  int halves, rows;          // of a workgroup: halves of wavefronts to a row, rows
   int rms;
   float eps_post, eps_pre, branch_scale, residual_scale, inv_K;
 };
@@ -75,82 +77,84 @@ struct Piece {
   }
 };
 
-// THREADS of a row: 64, a wavefront each and four of them to the workgroup; or the whole workgroup.  A thread holds NCH pieces of E values.
-// A row's threads go on to the rows behind it (a.run of them), keep the norms' weights and the gate in registers meanwhile and
-// request the next row before they work on this one (but 1024 threads, whose 128 registers hold no more than the row).
-template <class T, class R, int THREADS, int E, int NCH, bool BETAS>
-__global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void norm_residual_kernel(NormResidualArgs a) {
-  typedef Piece<unsigned short, E> P;
-  constexpr bool KEEP = THREADS < 1024;
-  constexpr int KEPT = KEEP ? NCH : 1;
-  constexpr int WAVES = THREADS / 64;
-  __shared__ float part[2][WAVES > 1 ? 4 * WAVES : 1];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row0 = (WAVES > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave) * a.run;
-  const int64_t end = min(row0 + a.run, a.M);
-  if (row0 >= end) return;
-  const int first = (WAVES > 1 ? (int)threadIdx.x : lane) * E;
-  const int K = a.K;
-  auto at = [&](int i) __attribute__((always_inline)) { return first + i * THREADS * E; };
+SF_DEVICE float half_sum(float v) {  // over 32 lanes: wave_reduce without its last step
+  v += dpp_f32<0xB1>(v);
+  v += dpp_f32<0x4E>(v);
+  v += dpp_f32<0x141>(v);
+  v += dpp_f32<0x140>(v);
+  typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+  const unsigned int b = __float_as_uint(v);
+  const u32x2_t r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
-  P gamma_post[KEPT], beta_post[BETAS ? KEPT : 1], gamma_pre[KEPT], beta_pre[BETAS ? KEPT : 1], gate[KEPT];
-  auto fetch = [&](P* to, const unsigned short* from) __attribute__((always_inline)) {
+// 32 lanes hold 256 NCH values of a row, and as many halves of wavefronts as that takes, `halves`, make up a row's threads: with an odd number
+// two rows share a workgroup and its middle wavefront (768 in pieces for a thread each: three halves).  A thread has NCH pieces of 16 bytes
+// (of 8: 65536 x 1280 238 us for 150).  What was behind that, all of it with fewer rows in flight: two rows to a thread, which then
+// share the norms' weights, 43008 x 2048 131 us for 133, but onto fp32, 21504 x 2048, 113 for 101; threads that go on to other rows with the weights kept in
+// registers, 65536 x 1280 143-180, 5003 x 8192 onto fp32 110-130.  The weights come out of the caches.
+template <class T, class R, int NCH>
+__global__ __launch_bounds__(1024) void norm_residual_kernel(NormResidualArgs a) {
+  constexpr int E = 8;
+  typedef Piece<unsigned short, E> P;
+  __shared__ float part[4][32];
+  const int lane = threadIdx.x & 63, half = (int)threadIdx.x >> 5;
+  const int mine = half >= a.halves;  // which of the workgroup's rows
+  const int64_t row = (int64_t)blockIdx.x * a.rows + mine;
+  const bool idle = half >= a.rows * a.halves || row >= a.M;  // (it meets the others at the barriers)
+  const int threads = 32 * a.halves, K = idle ? 0 : a.K;
+  const int first = ((int)threadIdx.x - mine * threads) * E;
+  auto at = [&](int i) __attribute__((always_inline)) { return first + i * threads * E; };
+
+  // everything is requested before anything is waited for, if there are registers for it
+  constexpr bool AHEAD = NCH <= 2;
+  const unsigned short* gate = a.gate ? a.gate + row / a.group * K : nullptr;
+  const unsigned short* const from[5] = {a.gamma_post, a.beta_post, gate, a.gamma_pre, a.beta_pre};
+  P ahead[AHEAD ? 5 : 1][NCH];
+  Piece<unsigned short, E> xw[NCH];
+  Piece<R, E> rw[NCH];
 #pragma unroll
-    for (int i = 0; i < KEPT; ++i)
-      if (at(i) < K) to[i].load(from + at(i), K - at(i));
-  };
-  auto piece = [&](const P* kept, const unsigned short* from, int i) __attribute__((always_inline)) {
-    if constexpr (KEEP) return kept[i];
+  for (int i = 0; i < NCH; ++i) {
+    if (at(i) < K) {
+      xw[i].load(a.x + row * a.ldx + at(i), K - at(i));
+      rw[i].load(reinterpret_cast<const R*>(a.residual) + row * a.ld_res + at(i), K - at(i));
+    } else {
+      xw[i] = {};
+      rw[i] = {};
+    }
+  }
+  if constexpr (AHEAD) {
+#pragma unroll
+    for (int j = 0; j < 5; ++j)
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        if (from[j] && at(i) < K) ahead[j][i].load(from[j] + at(i), K - at(i));
+  }
+  auto weights = [&](int j, int i) __attribute__((always_inline)) {
+    if constexpr (AHEAD) return ahead[j][i];
     P p;
-    p.load(from + at(i), K - at(i));
+    p.load(from[j] + at(i), K - at(i));
     return p;
   };
-  Piece<unsigned short, E> xn[NCH];
-  Piece<R, E> rn[NCH];
-  auto request = [&](int64_t row) __attribute__((always_inline)) {
-    const unsigned short* xs = a.x + row * a.ldx;
-    const R* rs = reinterpret_cast<const R*>(a.residual) + row * a.ld_res;
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      if (at(i) < K) {
-        xn[i].load(xs + at(i), K - at(i));
-        rn[i].load(rs + at(i), K - at(i));
-      } else {
-        xn[i] = {};
-        rn[i] = {};
-      }
-    }
-  };
-  request(row0);
-  if (KEEP && a.gamma_post) fetch(gamma_post, a.gamma_post);
-  if (KEEP && BETAS && a.beta_post) fetch(beta_post, a.beta_post);
-  if (KEEP && a.gamma_pre) fetch(gamma_pre, a.gamma_pre);
-  if (KEEP && BETAS && a.beta_pre) fetch(beta_pre, a.beta_pre);
 
   int round = 0;
-  // (the wavefronts' shares lie in places of their own for each of a row's four sums, and in another set for the next row: one barrier is enough)
-  auto sum = [&](float v, int set) __attribute__((always_inline)) {
-    v = wave_sum(v);
-    if constexpr (WAVES > 1) {
-      float* p = part[set] + WAVES * round++;
-      if (lane == 0) p[wave] = v;
-      __syncthreads();
-      v = 0.f;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) v += p[w];
-    }
-    return v;
+  auto sum = [&](float v) __attribute__((always_inline)) {
+    v = half_sum(v);
+    float* p = part[round++];  // (a place of its own for each of the four sums: no barrier behind the reading)
+    if ((lane & 31) == 0) p[half] = v;
+    __syncthreads();
+    return half_sum((lane & 31) < a.halves ? p[mine * a.halves + (lane & 31)] : 0.f);
   };
-  // f = the row's values; scaled to mean 0 (LayerNorm) and mean square 1, times gamma plus beta
-  auto norm = [&](float (&f)[NCH][E], const P* gamma, const unsigned short* gamma_at, const P* beta, const unsigned short* beta_at, float eps,
-                  int set) __attribute__((always_inline)) {
+  // f = the row's values; scaled to mean 0 (LayerNorm) and mean square 1, times weights(j) plus weights(j + 1)
+  float f[NCH][E];
+  auto norm = [&](int j, float eps) __attribute__((always_inline)) {
     if (!a.rms) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
         for (int e = 0; e < E; ++e) s += f[i][e];
-      const float mean = sum(s, set) * a.inv_K;
+      const float mean = sum(s) * a.inv_K;
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
@@ -161,101 +165,73 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void norm_residual_k
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
       for (int e = 0; e < E; ++e) q = fmaf(f[i][e], f[i][e], q);
-    const float scale = 1.0f / sqrtf(fmaf(sum(q, set), a.inv_K, eps));
+    const float scale = 1.0f / sqrtf(fmaf(sum(q), a.inv_K, eps));
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       if (at(i) >= K) continue;  // (what lies there stays 0)
-      const P g = piece(gamma, gamma_at, i);
+      const P g = weights(j, i);
 #pragma unroll
       for (int e = 0; e < E; ++e) f[i][e] = f[i][e] * scale * g.template get<T>(e);
-      if (BETAS && beta_at) {
-        const P b = piece(beta, beta_at, i);
+      if (from[j + 1]) {
+        const P b = weights(j + 1, i);
 #pragma unroll
         for (int e = 0; e < E; ++e) f[i][e] += b.template get<T>(e);
       }
     }
   };
 
-  int64_t gate_row = -1, gate_end = row0;  // the rows up to gate_end share the gate in registers
-  for (int64_t row = row0; row < end; ++row) {
-    float f[NCH][E];
-    Piece<R, E> rc[NCH];
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      rc[i] = rn[i];
+  for (int i = 0; i < NCH; ++i)
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[i][e] = xn[i].template get<T>(e);
+    for (int e = 0; e < E; ++e) f[i][e] = xw[i].template get<T>(e);
+  if (a.gamma_post) norm(0, a.eps_post);
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    if (at(i) >= K) continue;
+    if (gate) {
+      const P g = weights(2, i);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[i][e] *= g.template get<T>(e);
     }
-    if (a.gate && row >= gate_end) {
-      gate_row = row / a.group;
-      gate_end = (gate_row + 1) * a.group;
-      if (KEEP) fetch(gate, a.gate + gate_row * K);
-    }
-    if (KEEP && row + 1 < end) request(row + 1);
-    round = 0;
-    const int set = (int)(row - row0) & 1;
-    if (a.gamma_post) norm(f, gamma_post, a.gamma_post, beta_post, a.beta_post, a.eps_post, set);
-    R* total = reinterpret_cast<R*>(a.total) + row * K;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      if (at(i) >= K) continue;
-      P g = {};
-      if (a.gate) g = piece(gate, a.gate + gate_row * K, i);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float v = a.gate ? f[i][e] * g.template get<T>(e) : f[i][e];
-        f[i][e] = fmaf(a.residual_scale, rc[i].template get<T>(e), a.branch_scale * v);
-        if (at(i) + e >= K) f[i][e] = 0.f;
-      }
-      Piece<R, E> o;
-      o.template put<T>(f[i]);
-      o.store(total + at(i), K - at(i));
+    for (int e = 0; e < E; ++e) {
+      f[i][e] = fmaf(a.residual_scale, rw[i].template get<T>(e), a.branch_scale * f[i][e]);
+      if (at(i) + e >= K) f[i][e] = 0.f;
     }
-    if (a.normed) {
-      norm(f, gamma_pre, a.gamma_pre, beta_pre, a.beta_pre, a.eps_pre, set);
+    Piece<R, E> o;
+    o.template put<T>(f[i]);
+    o.store(reinterpret_cast<R*>(a.total) + row * K + at(i), K - at(i));
+  }
+  if (!a.normed) return;
+  norm(3, a.eps_pre);
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        if (at(i) >= K) continue;
-        P o;
-        o.template put<T>(f[i]);
-        o.store(a.normed + row * K + at(i), K - at(i));
-      }
-    }
-    if (!KEEP && row + 1 < end) request(row + 1);
+  for (int i = 0; i < NCH; ++i) {
+    if (at(i) >= K) continue;
+    P o;
+    o.template put<T>(f[i]);
+    o.store(a.normed + row * K + at(i), K - at(i));
   }
 }
 
-template <class T, class R, bool BETAS>
+template <class T, class R>
 static int launch_norm_residual(NormResidualArgs a, hipStream_t stream) {
-  using std::integral_constant;
-  // `keep` rows' threads fill the CUs' registers: as many runs of rows as that, all of them as long as one another
-  auto go = [&](auto threads, auto e, auto nch, int64_t keep) {
-    constexpr int TH = decltype(threads)::value;
-    a.run = (a.M + keep - 1) / keep;
-    const int64_t runs = (a.M + a.run - 1) / a.run;
-    const dim3 grid((unsigned int)(TH == 64 ? (runs + 3) / 4 : runs)), block(TH == 64 ? 256 : TH);
-    hipLaunchKernelGGL((norm_residual_kernel<T, R, TH, decltype(e)::value, decltype(nch)::value, BETAS>), grid, block, 0, stream, a);
+  auto go = [&](auto nch) {
+    constexpr int NCH = decltype(nch)::value;
+    a.halves = (a.K + 256 * NCH - 1) / (256 * NCH);
+    a.rows = a.halves % 2 == 1 && a.halves <= 15 ? 2 : 1;
+    const dim3 grid((unsigned int)((a.M + a.rows - 1) / a.rows)), block((a.rows * a.halves + 1) / 2 * 64);
+    hipLaunchKernelGGL((norm_residual_kernel<T, R, NCH>), grid, block, 0, stream, a);
     return check_launch("norm_residual_kernel");
   };
-  using E4 = integral_constant<int, 4>;
-  using E8 = integral_constant<int, 8>;
-  using N1 = integral_constant<int, 1>;
-  using N2 = integral_constant<int, 2>;
-  using N3 = integral_constant<int, 3>;
-  using N4 = integral_constant<int, 4>;
-  using N5 = integral_constant<int, 5>;
-  using T1 = integral_constant<int, 64>;
-  using T4 = integral_constant<int, 256>;
-  using T16 = integral_constant<int, 1024>;
-  if (a.K <= 256) return go(T1{}, E4{}, N1{}, 8192);
-  if (a.K <= 512) return go(T1{}, E8{}, N1{}, 8192);
-  if (a.K <= 768) return go(T1{}, E4{}, N3{}, 4096);
-  if (a.K <= 1024) return go(T1{}, E8{}, N2{}, 4096);
-  if (a.K <= 1280) return go(T1{}, E4{}, N5{}, 4096);
-  if (a.K <= 2048) return go(T1{}, E8{}, N4{}, 3072);
-  if (a.K <= 4096) return go(T4{}, E8{}, N2{}, 1024);
-  if (a.K <= 8192) return go(T4{}, E8{}, N4{}, 768);
-  return go(T16{}, E8{}, N4{}, 256);
+  using N1 = std::integral_constant<int, 1>;
+  using N2 = std::integral_constant<int, 2>;
+  using N4 = std::integral_constant<int, 4>;
+  if (a.K > 16384) return go(N4{});
+  // One piece to a thread / two, us at 88 M values: fp32 residuals 2048 101 / 120, 8192 106 / 117 (RMS) and 115 / 121; half types with RMS
+  // norms 1024 117 / 124, 4096 121 / 127, but 5000 158 / 131, 8192 132 / 127, with LayerNorms 512 129 / 129, 768 136 / 144, but 1280 157 / 141, 4096 142 / 131,
+  // 8192 158 / 137, and rows that start at odd addresses, 333 359 / 283 and 304 / 230, 1999 279 / 245 and 241 / 206
+  const bool two = a.K > 8192 || (sizeof(R) == 2 && (a.K > 4096 || (a.K > 1024 && !a.rms) || (a.K > 256 && a.K % 8 != 0)));
+  return two ? go(N2{}) : go(N1{});
 }
 
 }  // namespace samfast
@@ -299,11 +275,6 @@ extern "C" int samfast_norm_residual(const void* x, int64_t ldx, const void* res
   a.residual_scale = residual_scale;
   a.inv_K = 1.0f / (float)K;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  auto go = [&](auto elem) {
-    using T = decltype(elem);
-    const bool betas = post_beta || pre_beta;
-    if (residual_is_f32) return betas ? launch_norm_residual<T, float, true>(a, s) : launch_norm_residual<T, float, false>(a, s);
-    return betas ? launch_norm_residual<T, us, true>(a, s) : launch_norm_residual<T, us, false>(a, s);
-  };
-  return dtype == SAMFAST_F16 ? go(ElemF16{}) : go(ElemBf16{});
+  if (dtype == SAMFAST_F16) return residual_is_f32 ? launch_norm_residual<ElemF16, float>(a, s) : launch_norm_residual<ElemF16, us>(a, s);
+  return residual_is_f32 ? launch_norm_residual<ElemBf16, float>(a, s) : launch_norm_residual<ElemBf16, us>(a, s);
 }

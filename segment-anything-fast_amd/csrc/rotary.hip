@@ -3,7 +3,7 @@
 // over the first `width` channels of a head, the others copied; one launch for queries and keys.
 //
 // Every value is read and written once, so memory bounds it.  An angle belongs to a token and a pair, not to a head: a workgroup takes a
-// few tokens, makes their cosines and sines once and goes through all the heads with them.  The angle is a product in 64 bits, in turns,
+// few tokens, makes their cosines and sines once and turns the heads with them, 32 to 64 bytes to a thread, all of them requested before the table is made.  The angle is a product in 64 bits, in turns,
 // of which only the fraction goes on in 32: at position 10^6 the 24 bits of a float product leave 1/16 of a radian.
 #include "samfast_internal.hpp"
 #include "attn_relpos_shared.hpp"
@@ -24,18 +24,19 @@ struct RotaryArgs {
   int64_t pos_b;
   float magnitude;
   int tokens, T, heads_q, heads, D, pairs, axes;
-  int items;                  // pieces of a head
-  int chunks, copies;         // halves: pieces of an axis, pieces that are only copied
+  int items;                  // a head's pieces; halves: the first `turns` of them are turned, `chunks` for an axis, the others copied
+  int chunks, turns;
   int block_tokens, block_heads;
-  unsigned int div_items, div_turned, div_copies, div_heads, div_chunks;  // 2^32 / d, rounded up: x / d is the upper half of a product where x d < 2^32
+  unsigned int div_items, div_heads;  // 2^32 / d, rounded up: x / d is the upper half of a product where x d < 2^32
 };
 
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryPiece = 8;       // channels (halves: pairs) of a piece
-constexpr int kRotaryItems = 2048;    // pieces of a workgroup, unless one head has more
+constexpr int kRotaryPiece = 8;       // values of 16 bytes
 constexpr int kRotaryTable = 1024;    // angles of a workgroup
 constexpr int kRotaryMaxDim = 1024;
-enum { kNeighbours, kHalves, kCopies };
+// cosine and sine of the workgroup's angle i: a lane reads PLANES adjacent ones, which lie apart so that its neighbours' lie side by side
+template <int PLANES>
+SF_DEVICE int table_at(int i) { return i % PLANES * (kRotaryTable / PLANES + 1) + i / PLANES; }
 
 SF_DEVICE u32x4 load_any(const unsigned short* p) {  // 16 bytes from any even address
   u32x4 v;
@@ -61,9 +62,12 @@ SF_DEVICE void store_some(unsigned short* p, u32x4 v, int n) {
 template <class T>
 SF_DEVICE float value(const u32x4& v, int e) { return e & 1 ? T::hi(v[e >> 1]) : T::lo(v[e >> 1]); }
 
-template <class T, bool INTERLEAVED>
+// EACH pieces of a thread
+template <class T, bool INTERLEAVED, int EACH>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
-  __shared__ f32x2 table[kRotaryTable];  // cosine and sine
+  constexpr int PLANES = INTERLEAVED ? 4 : 8;
+  static_assert(kRotaryMaxDim / kRotaryPiece <= EACH * kRotaryThreads, "a workgroup has whole heads");
+  __shared__ f32x2 table[kRotaryTable + PLANES];
   const int t0 = (int)blockIdx.x * a.block_tokens;
   const int nt = min(a.block_tokens, a.tokens - t0);
   const unsigned int b0 = (unsigned int)t0 / (unsigned int)a.T, first = (unsigned int)t0 - b0 * (unsigned int)a.T;
@@ -80,109 +84,109 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   const int h0 = blockIdx.y * a.block_heads, nh = min(a.block_heads, a.heads - h0);
   const int angles = a.axes * a.pairs;
 
-  auto make_table = [&]() __attribute__((always_inline)) {
-    for (int i = threadIdx.x; i < nt * angles; i += kRotaryThreads) {
-      const int t = i / angles, p = i - t * angles;
-      int64_t b, n;
-      place(t, b, n);
-      const double pos = (double)a.pos[b * a.pos_b + n * a.axes + (a.axes == 1 ? 0 : p / a.pairs)];
-      double turns = pos * (a.freq[p] * 0.15915494309189535);  // 1 / 2 pi
-      turns -= rint(turns);
-      float s, c;
-      sincospif(2.0f * (float)turns, &s, &c);
-      table[i] = f32x2{c * a.magnitude, s * a.magnitude};
+  // What a thread has of a head at a time: kRotaryPiece channels (neighbours), or as many pairs of halves, lower and upper channels, or twice
+  // as many channels that are only copied
+  struct Where {
+    const unsigned short* in;
+    unsigned short* out;
+    int angle, turned;  // its first angle, and how many pairs from there on are turned
+    int n, second, n2;  // values of the first 16 bytes, where the second ones start, values of these
+  };
+  const unsigned int total = (unsigned int)(nt * nh * a.items);
+  auto where = [&](unsigned int i) __attribute__((always_inline)) {
+    Where w = {};
+    if (i >= total) return w;
+    const unsigned int row = a.items == 1 ? i : __umulhi(i, a.div_items);
+    const int item = (int)(i - row * a.items);
+    const int t = a.block_heads == 1 ? (int)row : (int)__umulhi(row, a.div_heads);  // (0 where heads are split: one token then)
+    int h = h0 + (int)row - t * nh;
+    int64_t b, token;
+    place(t, b, token);
+    const RotarySide& s = a.side[h >= a.heads_q];
+    if (h >= a.heads_q) h -= a.heads_q;
+    int d = item * kRotaryPiece;
+    w.angle = t * angles;
+    if (INTERLEAVED) {
+      w.n = min(kRotaryPiece, a.D - d);
+      w.angle += d / 2;
+      w.turned = angles - d / 2;
+    } else if (item < a.turns) {
+      const int axis = a.axes == 1 ? 0 : item / a.chunks;
+      const int p = d - axis * a.chunks * kRotaryPiece;
+      d = 2 * axis * a.pairs + p;
+      w.angle += axis * a.pairs + p;
+      w.turned = w.n = w.n2 = min(kRotaryPiece, a.pairs - p);
+      w.second = a.pairs;
+    } else {
+      d = 2 * angles + (item - a.turns) * 2 * kRotaryPiece;
+      w.n = min(kRotaryPiece, a.D - d);
+      w.second = kRotaryPiece;
+      w.n2 = max(min(kRotaryPiece, a.D - d - kRotaryPiece), 0);
     }
-    __syncthreads();
+    w.in = s.in + b * s.in_b + h * s.in_h + token * s.in_t + d;
+    w.out = s.out + b * s.out_b + h * s.out_h + token * s.out_t + d;
+    return w;
   };
 
-  // The pieces of one kind, `items` of them to a head, UNROLL of a thread at a time with all their loads in flight; before the first are used,
-  // `ready` is called.
-  auto walk = [&](auto kind, unsigned int items, unsigned int div, auto ready) __attribute__((always_inline)) {
-    constexpr int KIND = decltype(kind)::value;
-    constexpr int UNROLL = KIND == kHalves ? 2 : 4;
-    const unsigned int total = (unsigned int)(nt * nh) * items;
-    bool first_round = true;
-    for (unsigned int i0 = threadIdx.x; first_round || i0 < total; i0 += UNROLL * kRotaryThreads) {
-      u32x4 x[UNROLL], y[UNROLL];
-      unsigned short* out[UNROLL];
-      int at[UNROLL], n[UNROLL], turned[UNROLL];  // first angle, channels (halves: pairs), neighbours: pairs from here on that are turned
+  // all loads are under way before the table is made
+  u32x4 x[EACH], y[EACH];
+  Where w[EACH];
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const unsigned int i = i0 + u * kRotaryThreads;
-        n[u] = 0;
-        if (i >= total) continue;
-        const unsigned int row = items == 1 ? i : __umulhi(i, div);
-        const int item = (int)(i - row * items);
-        const int t = a.block_heads == 1 ? (int)row : (int)__umulhi(row, a.div_heads);  // (0 where heads are split: one token then)
-        int h = h0 + (int)row - t * nh;
-        int64_t b, token;
-        place(t, b, token);
-        const RotarySide& s = a.side[h >= a.heads_q];
-        if (h >= a.heads_q) h -= a.heads_q;
-        int d = item * kRotaryPiece;
-        at[u] = t * angles + d / 2;
-        turned[u] = angles - d / 2;
-        if (KIND == kHalves) {
-          const int axis = a.axes == 1 ? 0 : a.chunks == 1 ? item : (int)__umulhi((unsigned int)item, a.div_chunks);
-          const int p = d - axis * a.chunks * kRotaryPiece;
-          n[u] = min(kRotaryPiece, a.pairs - p);
-          at[u] = t * angles + axis * a.pairs + p;
-          d = 2 * axis * a.pairs + p;
-        } else {
-          if (KIND == kCopies) d += 2 * angles;
-          n[u] = min(kRotaryPiece, a.D - d);
-        }
-        const unsigned short* in = s.in + b * s.in_b + h * s.in_h + token * s.in_t + d;
-        out[u] = s.out + b * s.out_b + h * s.out_h + token * s.out_t + d;
-        x[u] = load_some(in, n[u]);
-        if (KIND == kHalves) y[u] = load_some(in + a.pairs, n[u]);
+  for (int u = 0; u < EACH; ++u) {
+    w[u] = where(threadIdx.x + u * kRotaryThreads);
+    x[u] = y[u] = u32x4{};
+    if (w[u].n > 0) x[u] = load_some(w[u].in, w[u].n);
+    if (!INTERLEAVED && w[u].n2 > 0) y[u] = load_some(w[u].in + w[u].second, w[u].n2);
+  }
+  for (int i = threadIdx.x; i < nt * angles; i += kRotaryThreads) {
+    const int t = i / angles, p = i - t * angles;
+    int64_t b, n;
+    place(t, b, n);
+    const double pos = (double)a.pos[b * a.pos_b + n * a.axes + (a.axes == 1 ? 0 : p / a.pairs)];
+    double turns = pos * (a.freq[p] * 0.15915494309189535);  // 1 / 2 pi
+    turns -= rint(turns);
+    float s, c;
+    sincospif(2.0f * (float)turns, &s, &c);
+    table[table_at<PLANES>(i)] = f32x2{c * a.magnitude, s * a.magnitude};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {
+    if (w[u].n == 0) continue;
+    if (INTERLEAVED) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool turned = j < w[u].turned;
+        const f32x2 c = table[table_at<PLANES>(turned ? w[u].angle + j : 0)];
+        const float v0 = T::lo(x[u][j]), v1 = T::hi(x[u][j]);
+        if (turned) x[u][j] = T::pack2(v0 * c[0] - v1 * c[1], v1 * c[0] + v0 * c[1]);
       }
-      if (first_round) ready();
-      first_round = false;
+    } else if (w[u].turned > 0) {
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        if (n[u] == 0) continue;
-        if (KIND == kNeighbours) {
-          u32x4 o;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x2 w = table[j < turned[u] ? at[u] + j : 0];
-            const float v0 = T::lo(x[u][j]), v1 = T::hi(x[u][j]);
-            o[j] = j < turned[u] ? T::pack2(v0 * w[0] - v1 * w[1], v1 * w[0] + v0 * w[1]) : x[u][j];
-          }
-          store_some(out[u], o, n[u]);
-        } else if (KIND == kHalves) {
-          u32x4 ox, oy;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x2 w0 = table[at[u] + min(2 * j, n[u] - 1)], w1 = table[at[u] + min(2 * j + 1, n[u] - 1)];
-            const float x0 = T::lo(x[u][j]), x1 = T::hi(x[u][j]), y0 = T::lo(y[u][j]), y1 = T::hi(y[u][j]);
-            ox[j] = T::pack2(x0 * w0[0] - y0 * w0[1], x1 * w1[0] - y1 * w1[1]);
-            oy[j] = T::pack2(y0 * w0[0] + x0 * w0[1], y1 * w1[0] + x1 * w1[1]);
-          }
-          store_some(out[u], ox, n[u]);
-          store_some(out[u] + a.pairs, oy, n[u]);
-        } else {
-          store_some(out[u], x[u], n[u]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const f32x2 c0 = table[table_at<PLANES>(w[u].angle + min(2 * j, w[u].turned - 1))];
+        const f32x2 c1 = table[table_at<PLANES>(w[u].angle + min(2 * j + 1, w[u].turned - 1))];
+        const float x0 = T::lo(x[u][j]), x1 = T::hi(x[u][j]), y0 = T::lo(y[u][j]), y1 = T::hi(y[u][j]);
+        x[u][j] = T::pack2(x0 * c0[0] - y0 * c0[1], x1 * c1[0] - y1 * c1[1]);
+        y[u][j] = T::pack2(y0 * c0[0] + x0 * c0[1], y1 * c1[0] + x1 * c1[1]);
       }
     }
-  };
-  if (INTERLEAVED) {
-    walk(std::integral_constant<int, kNeighbours>{}, (unsigned int)a.items, a.div_items, make_table);
-  } else {
-    walk(std::integral_constant<int, kHalves>{}, (unsigned int)(a.axes * a.chunks), a.div_turned, make_table);
-    if (a.copies > 0) walk(std::integral_constant<int, kCopies>{}, (unsigned int)a.copies, a.div_copies, [] {});
+    store_some(w[u].out, x[u], w[u].n);
+    if (!INTERLEAVED && w[u].n2 > 0) store_some(w[u].out + w[u].second, y[u], w[u].n2);
   }
 }
 
 static unsigned int divider(int d) { return (unsigned int)(((uint64_t)1 << 32) / (unsigned int)d + 1); }  // (d > 1)
 
+// Pieces of a thread.  Neighbours 2 / 4: 16 x 4096 tokens, 32 heads of 80 194 / 127 us, 8 x 4096, 40 of 128 162 / 124; halves 1 / 2 / 4: 129 / 143 /
+// 143, 126 / 125 / 129, 30011 tokens, 28 heads, 64 of 96 channels 59 / 64 / 67.
+constexpr int kRotaryNeighbours = 4, kRotaryHalves = 1;
+
 template <class T>
 static int launch_rotary(RotaryArgs a, bool interleaved, hipStream_t stream) {
   const dim3 grid((unsigned int)((a.tokens + a.block_tokens - 1) / a.block_tokens), (unsigned int)((a.heads + a.block_heads - 1) / a.block_heads));
-  if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, true>), grid, dim3(kRotaryThreads), 0, stream, a);
-  else hipLaunchKernelGGL((rotary_kernel<T, false>), grid, dim3(kRotaryThreads), 0, stream, a);
+  if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, true, kRotaryNeighbours>), grid, dim3(kRotaryThreads), 0, stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<T, false, kRotaryHalves>), grid, dim3(kRotaryThreads), 0, stream, a);
   return check_launch("rotary_kernel");
 }
 
@@ -221,11 +225,12 @@ extern "C" int samfast_rotary(const void* q, const void* k, void* q_out, void* k
   a.axes = axes;
   const int angles = axes * pairs;
   a.chunks = (pairs + kRotaryPiece - 1) / kRotaryPiece;
-  a.copies = (D - 2 * angles + kRotaryPiece - 1) / kRotaryPiece;
-  a.items = interleaved ? (D + kRotaryPiece - 1) / kRotaryPiece : axes * a.chunks + a.copies;
-  // a workgroup's share: kRotaryItems pieces, fewer where that leaves CUs without one
+  a.turns = axes * a.chunks;
+  a.items = interleaved ? (D + kRotaryPiece - 1) / kRotaryPiece : a.turns + (D - 2 * angles + 2 * kRotaryPiece - 1) / (2 * kRotaryPiece);
+  // a workgroup's share: what its threads hold at most, fewer where that leaves CUs without one
+  const int64_t most = (interleaved ? kRotaryNeighbours : kRotaryHalves) * kRotaryThreads;
   int64_t share = (int64_t)a.tokens * a.heads * a.items / 1024;
-  share = share < kRotaryThreads ? kRotaryThreads : share > kRotaryItems ? kRotaryItems : share;
+  share = share < kRotaryThreads ? kRotaryThreads : share > most ? most : share;
   int64_t heads = share / a.items;
   a.block_heads = (int)(heads < 1 ? 1 : heads > a.heads ? a.heads : heads);
   const int parts = (a.heads + a.block_heads - 1) / a.block_heads;
@@ -235,10 +240,7 @@ extern "C" int samfast_rotary(const void* q, const void* k, void* q_out, void* k
   a.block_tokens = (int)(tokens < 1 ? 1 : tokens);
   SF_REQUIRE(parts < 65536, "rotary: too many heads");
   a.div_items = a.items > 1 ? divider(a.items) : 0;
-  a.div_turned = axes * a.chunks > 1 ? divider(axes * a.chunks) : 0;
-  a.div_copies = a.copies > 1 ? divider(a.copies) : 0;
   a.div_heads = a.block_heads > 1 ? divider(a.block_heads) : 0;
-  a.div_chunks = a.chunks > 1 ? divider(a.chunks) : 0;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return dtype == SAMFAST_F16 ? launch_rotary<ElemF16>(a, interleaved != 0, s) : launch_rotary<ElemBf16>(a, interleaved != 0, s);
 }
