@@ -249,7 +249,7 @@ int samfast_linear_half(
  * Over more than SAMFAST_I4_FEW_ROWS rows the weights (code - zero) * scale are rounded to `dtype` before they are
  * multiplied: in fp16 they have to stay below 65504 there.
  */
-#define SAMFAST_I4_FEW_ROWS 64
+#define SAMFAST_I4_FEW_ROWS 32
 int64_t samfast_linear_i4_workspace(int64_t M, int N, int K);
 int samfast_linear_i4(
     const void* x, int64_t ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros, const float* bias,

@@ -156,6 +156,42 @@ __global__ __launch_bounds__(256, 2) void linear_i4_tiled_kernel(I4Args a) {
   }
 }
 
+// y = the parts' sums + bias: four columns a thread
+template <class T>
+__global__ __launch_bounds__(256) void i4_sum_kernel(I4Args a, int splits) {
+  const int quads = (a.N + 3) / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.M * quads) return;
+  const int m = (int)(i / quads), n = 4 * (int)(i - (int64_t)m * quads);
+  float v[4] = {};
+  const float* part = a.parts + (int64_t)m * a.N + n;
+  if (n + 4 <= a.N) {
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      float p[4];
+      __builtin_memcpy(p, part + (int64_t)s * a.M * a.N, 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += p[e];
+    }
+  } else {
+    for (int s = 0; s < splits; ++s)
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (n + e < a.N) v[e] += part[(int64_t)s * a.M * a.N + e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] += a.bias ? a.bias[min(n + e, a.N - 1)] : 0.f;
+  const u32x2 r = {T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
+  unsigned short* y = a.y + (int64_t)m * a.ldy + n;
+  if (n + 4 <= a.N) {
+    __builtin_memcpy(y, &r, 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (n + e < a.N) y[e] = (unsigned short)(r[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
 template <class T>
 static int launch_i4_tiled(I4Args a, hipStream_t stream) {
   auto go = [&](auto fm, auto fn) {
@@ -186,7 +222,7 @@ extern "C" int samfast_linear_i4(const void* x, int64_t ldx, const uint8_t* code
   if (dtype != SAMFAST_BF16 && dtype != SAMFAST_F16) SF_FAIL(SAMFAST_E_UNSUPPORTED, "linear_i4: element type %d is neither SAMFAST_BF16 nor SAMFAST_F16", dtype);
   SF_REQUIRE(M >= 0 && N > 0 && K > 0 && K % 8 == 0, "linear_i4: bad shape M=%lld N=%d K=%d (K must be a multiple of 8)", (long long)M, N, K);
   SF_REQUIRE(group > 0 && group % 32 == 0, "linear_i4: groups of %d inputs (must be a multiple of 32)", group);
-  SF_REQUIRE(M < (1ll << 31) - 512 && N < (1 << 30) && K < (1 << 22) && ldx < (1 << 22), "linear_i4: too large");
+  SF_REQUIRE(M < (1ll << 31) - 512 && N < (1 << 30) && K <= kI4MaxInputs && ldx < (1 << 22), "linear_i4: too large");
   SF_REQUIRE(((M + 63) / 64) * ((N + 63) / 64) < (1ll << 31) - 8, "linear_i4: too large");
   if (M == 0) return SAMFAST_OK;
   SF_REQUIRE(x && codes && scales && y, "linear_i4: null pointer");
@@ -206,10 +242,11 @@ extern "C" int samfast_linear_i4(const void* x, int64_t ldx, const uint8_t* code
   a.N = N;
   a.K = K;
   a.group = group;
+  a.div_group = i4_divider(group < K ? group : (K + 31) / 32 * 32);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int tile = i4_dense_tile(M, N, K);
   SF_REQUIRE(tile == 0 || (workspace && aligned16(workspace)), "linear_i4: this shape needs a 16-byte aligned workspace (samfast_linear_i4_workspace)");
   if (tile != 0 && ldy % 8 == 0 && ldy < (1 << 22) && aligned16(y)) return launch_i4_dense(a, dtype == SAMFAST_F16, tile, workspace, s);
-  if (M <= SAMFAST_I4_FEW_ROWS) return launch_i4_few(a, dtype == SAMFAST_F16, s);
+  if (M <= SAMFAST_I4_FEW_ROWS && N >= 16) return launch_i4_few(a, dtype == SAMFAST_F16, s);
   return dtype == SAMFAST_F16 ? launch_i4_tiled<ElemF16>(a, s) : launch_i4_tiled<ElemBf16>(a, s);
 }

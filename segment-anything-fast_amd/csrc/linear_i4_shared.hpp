@@ -14,10 +14,17 @@ struct I4Args {
   const unsigned char* zeros;    // (groups, N), or null: 8 throughout
   const float* bias;             // (N), or null
   unsigned short* y;             // (M, N), row stride ldy
+  float* parts;                  // K split between workgroups: their sums (splits, M, N); else null
   int64_t ldx, ldy;
   int M, N, K, group;            // K % 8 == 0, group % 32 == 0
+  unsigned int div_group;        // for i4_group
   int tiles_m, tiles_n;
 };
+
+// The group of the 32 inputs from 32 * step on: step / (group / 32), exact below 2^15 steps, which K <= kI4MaxInputs keeps
+constexpr int kI4MaxInputs = 1 << 20;
+static inline unsigned int i4_divider(int group) { return (unsigned int)((((uint64_t)1 << 31) + group / 32 - 1) / (group / 32)); }
+SF_DEVICE int i4_group(const I4Args& a, int step) { return (int)__umulhi((unsigned int)(2 * step), a.div_group); }
 
 // The eight codes of a word in the order of k, as floats 0 to 15: the even and the odd ones stand in bytes of their own for
 // v_cvt_f32_ubyte.
