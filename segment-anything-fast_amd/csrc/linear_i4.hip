@@ -1,20 +1,9 @@
-// Linears with 4-bit weights over many rows: a tiled matrix product that makes the weights of a tile, rounded to the element type, on
-// their way into LDS.
+// Linears with 4-bit weights over more than a few rows, of any shape: a tiled matrix product whose wavefronts make their own weights.
 #include "linear_i4_shared.hpp"
 
+#include <type_traits>
+
 namespace samfast {
-
-template <class T, int FM, int FN>
-struct I4Tile {
-  static constexpr int BM = 32 * FM, BN = 32 * FN;   // four wavefronts, two by two, of FM x FN fragments of 16 x 16
-  static constexpr int STAGE = (BM + BN) * 128;      // one k tile of 64 of both operands
-  static constexpr int KT = BN / 4;                  // values of a weight tile that a thread makes: 256 threads, 64 BN values
-  static constexpr int WORDS = KT / 8;
-  static constexpr int THREADS_ROW = 64 / KT;        // threads that share a row
-};
-
-// 16-byte piece c of LDS row r stands at position c ^ ((r >> 1) & 7): a fragment's read (16 rows, four pieces) touches every bank once
-SF_DEVICE int i4_place(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) << 4); }
 
 // 16 bytes a lane from base + offset to lds + 16 lane; zeros where the offset is kOutside
 constexpr unsigned int kOutside = 0x80000000u;
@@ -23,134 +12,241 @@ SF_DEVICE void piece_to_lds(const void* base, unsigned int offset, void* lds) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, offset, 0, 0, 0);
 }
 
-template <class T, int FM, int FN>
-__global__ __launch_bounds__(256, 2) void linear_i4_tiled_kernel(I4Args a) {
-  using P = I4Tile<T, FM, FN>;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * P::STAGE];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave & 1, wn = wave >> 1, lr = lane & 15, lq = lane >> 4;
+// The eight weights (code - zero) * scale of a word in the order of k, rounded to the element type once: code - zero is exact, and so is
+// zero * scale in fp32.
+SF_DEVICE u32x4 i4_weights(ElemBf16, unsigned int w, float scale, float zero) {
+  const u32x2 bytes = i4_bytes(w);
+  const float off = -zero * scale;
+  u32x4 o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(bytes[h], 512.f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(bytes[h], 512.f, true);
+    o[2 * h] = ElemBf16::pack2(fmaf(lo[0], scale, off), fmaf(lo[1], scale, off));
+    o[2 * h + 1] = ElemBf16::pack2(fmaf(hi[0], scale, off), fmaf(hi[1], scale, off));
+  }
+  return o;
+}
+SF_DEVICE u32x4 i4_weights(ElemF16, unsigned int w, float scale, float zero) {
+  typedef ElemF16::f16x2 f16x2;
+  const u32x2 bytes = i4_bytes(w);
+  const f16x2 s = {(_Float16)scale, (_Float16)scale}, z = {(_Float16)zero, (_Float16)zero};
+  u32x4 o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    o[2 * h] = __builtin_bit_cast(unsigned int, (__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes[h], 512.f, false) - z) * s);
+    o[2 * h + 1] = __builtin_bit_cast(unsigned int, (__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes[h], 512.f, true) - z) * s);
+  }
+  return o;
+}
 
-  // neighbours on an XCD share the weights' tile columns in groups of eight rows of tiles
+// Tiles of 16 MT rows and 16 NT WAVES columns, K 128 at a time.  The rows of x are everybody's and go through LDS, STAGES k tiles of them; the columns
+// are one wavefront's each, so that a weight is made once in the workgroup and never leaves the registers.
+template <int MT, int NT, int WAVES, int STAGES>
+struct I4Tile {
+  static constexpr int BM = 16 * MT, BN = 16 * NT * WAVES, STAGE = BM * 256;
+  static constexpr int LOADS = 4 * MT / WAVES;  // of a wavefront for a k tile of x: eight rows' lines each
+  static constexpr int ISSUED = LOADS + 2 * NT;  // with codes and scales (zeros not counted: then a few more have landed than need be)
+  static_assert(4 * MT % WAVES == 0 && STAGES * STAGE <= 160 * 1024 && (STAGES - 1) * ISSUED < 64, "");
+};
+
+template <class T, int MT, int NT, int WAVES, int STAGES>
+__global__ __launch_bounds__(64 * WAVES, 2) void linear_i4_kernel(I4Args a) {
+  using P = I4Tile<MT, NT, WAVES, STAGES>;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[STAGES * P::STAGE];
+  const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // neighbours on an XCD share a column of tiles, eight rows of them at a time
   const unsigned int total = (unsigned int)a.tiles_m * (unsigned int)a.tiles_n;
   const unsigned int pid = xcd_contiguous_id(blockIdx.x, total);
   if (pid >= total) return;
   const unsigned int per_group = 8u * a.tiles_n, first_m = pid / per_group * 8u;
   const unsigned int rows = min((unsigned int)a.tiles_m - first_m, 8u), in_group = pid % per_group;
-  const int m0 = (int)(first_m + in_group % rows) * P::BM, n0 = (int)(in_group / rows) * P::BN;
+  const int m0 = (int)(first_m + in_group % rows) * P::BM, n0 = (int)(in_group / rows) * P::BN + wave * 16 * NT;
+  // this workgroup's k tiles; the last one of all may end behind K
+  const int tiles = (a.K + 127) / 128;
+  const int first = (int)((int64_t)tiles * blockIdx.y / gridDim.y), end = (int)((int64_t)tiles * (blockIdx.y + 1) / gridDim.y);
 
-  // ---- x: 16-byte pieces straight into LDS; a piece outside the matrix gets an offset behind the buffer's end and arrives as zeros
-  constexpr int XLOADS = P::BM / 32;
-  unsigned int x_off[XLOADS];
-  int x_k[XLOADS];
+  // ---- x: a load puts eight rows' lines side by side; 16-byte piece c of row r stands at position c ^ ((r >> 1) & 7), where a fragment's read finds
+  // no two of its pieces in one bank.  What lies outside the matrix arrives as zeros.
+  unsigned int x_off[P::LOADS];
+  int x_k[P::LOADS];
 #pragma unroll
-  for (int i = 0; i < XLOADS; ++i) {
-    const int row = (wave + 4 * i) * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
-    x_k[i] = piece * 8;
-    x_off[i] = m0 + row < a.M ? (unsigned int)row * (unsigned int)(a.ldx * 2) + piece * 16 : kOutside;
+  for (int i = 0; i < P::LOADS; ++i) {
+    const int q = wave + WAVES * i, row = 8 * (q % (2 * MT)) + (lane >> 3);
+    x_k[i] = q / (2 * MT) * 64 + ((lane & 7) ^ ((row >> 1) & 7)) * 8;
+    x_off[i] = m0 + row < a.M ? (unsigned int)row * (unsigned int)(a.ldx * 2) + 2 * x_k[i] : kOutside;
   }
   const unsigned short* xt = a.x + (int64_t)m0 * a.ldx;
-  auto load_x = [&](int k0, int stage) __attribute__((always_inline)) {
+  auto load_x = [&](int kt, int stage) __attribute__((always_inline)) {
+    unsigned char* to = lds + stage * P::STAGE;
 #pragma unroll
-    for (int i = 0; i < XLOADS; ++i) piece_to_lds(xt + k0, k0 + x_k[i] < a.K ? x_off[i] : kOutside, lds + stage + (wave + 4 * i) * 1024);
+    for (int i = 0; i < P::LOADS; ++i) piece_to_lds(xt + kt * 128, kt * 128 + x_k[i] < a.K ? x_off[i] : kOutside, to + (wave + WAVES * i) * 1024);
+  };
+  auto x_piece = [&](int stage, int i, int t) __attribute__((always_inline)) {
+    const int row = 16 * i + lr, c = 4 * (t & 1) + lq;
+    return *reinterpret_cast<const u32x4*>(lds + stage * P::STAGE + (t >> 1) * P::BM * 128 + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
   };
 
-  // ---- weights: a thread's KT codes of one row.  Row i of fragment j of a wavefront's 16 FN columns holds column
-  // 4 FN (i / 4) + 4 j + i % 4, so that a lane ends with 4 FN adjacent ones.
-  const int wrow = tid / P::THREADS_ROW, wk = tid % P::THREADS_ROW * P::KT;
-  const int in_wave = wrow % (16 * FN), wi = in_wave % 16, wj = in_wave / 16;
-  const int wcol = min(n0 + wrow / (16 * FN) * 16 * FN + 4 * FN * (wi >> 2) + 4 * wj + (wi & 3), a.N - 1);
-  const unsigned char* wcodes = a.codes + (int64_t)wcol * (a.K / 2);
-  unsigned int cw[P::WORDS];
-  unsigned int csw, czw;
-  auto load_w = [&](int k0) __attribute__((always_inline)) {
-    const int k = k0 + wk;
-    if (k + P::KT <= a.K) {
-      __builtin_memcpy(cw, __builtin_assume_aligned(wcodes + k / 2, 4), P::KT / 2);
-    } else {
+  // ---- weights: row r of fragment j holds column 4 NT (r / 4) + 4 j + r % 4, so that a lane ends with 4 NT adjacent ones.  A lane has its
+  // column's 32 adjacent codes, and the scale and zero of the group that the 32 inputs of quarter lq belong to.
+  struct Weights {
+    u32x4 codes[NT];
+    unsigned int scale[NT], zero[NT];
+  };
+  int col[NT];
 #pragma unroll
-      for (int j = 0; j < P::WORDS; ++j) {
-        cw[j] = 0;
-        if (k + 8 * j < a.K) __builtin_memcpy(&cw[j], __builtin_assume_aligned(wcodes + k / 2 + 4 * j, 4), 4);
+  for (int j = 0; j < NT; ++j) col[j] = min(n0 + 4 * NT * (lr >> 2) + 4 * j + (lr & 3), a.N - 1);
+  auto load_w = [&](Weights& w, int kt) __attribute__((always_inline)) {
+    const int64_t at = (int64_t)i4_group(a, min(4 * kt + lq, (a.K - 1) / 32)) * a.N;
+    const unsigned char* zeros = a.zeros ? a.zeros : a.codes;  // (without zeros: not used)
+    const int64_t zero_at = a.zeros ? at : 0;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      __builtin_memcpy(&w.codes[j], __builtin_assume_aligned(a.codes + (int64_t)col[j] * (a.K / 2) + kt * 64 + 16 * lq, 4), 16);
+      w.scale[j] = a.scales[at + col[j]];
+      w.zero[j] = zeros[zero_at + col[j]];
+    }
+  };
+  auto load_w_careful = [&](Weights& w, int kt) __attribute__((always_inline)) {  // the k tile that may end behind K
+    const int64_t at = (int64_t)i4_group(a, min(4 * kt + lq, (a.K - 1) / 32)) * a.N;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      w.codes[j] = u32x4{};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (kt * 128 + 32 * lq + 8 * e < a.K) w.codes[j][e] = *reinterpret_cast<const unsigned int*>(a.codes + (int64_t)col[j] * (a.K / 2) + kt * 64 + 16 * lq + 4 * e);
+      w.scale[j] = a.scales[at + col[j]];
+      w.zero[j] = a.zeros ? a.zeros[at + col[j]] : 0;
+    }
+  };
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{};
+  auto multiply = [&](const Weights& w, int stage) __attribute__((always_inline)) {
+    u32x4 c[NT];
+    unsigned int sz[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      c[j] = w.codes[j];
+      i4_transpose(c[j]);
+      sz[j] = w.scale[j] | (a.zeros ? w.zero[j] : 8u) << 24;  // (to the top: of a byte in a register nothing has to be cleared before it is loaded)
+    }
+    u32x4 x[2][MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[0][i] = x_piece(stage, i, 0);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (t < 3) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[(t + 1) & 1][i] = x_piece(stage, i, t + 1);
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const unsigned int g = (unsigned int)__builtin_amdgcn_ds_bpermute(4 * (16 * t + lr), (int)sz[j]);
+        const u32x4 f = i4_weights(T{}, c[j][t], T::from_bits((unsigned short)g), (float)(g >> 24));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][j] = T::mfma16(f, x[t & 1][i], acc[i][j]);
       }
     }
-    const int64_t at = (int64_t)(min(k, a.K - 1) / a.group) * a.N + wcol;
-    csw = a.scales[at];
-    czw = a.zeros ? a.zeros[at] : 8u;
-  };
-  auto make_w = [&](int k0, int stage) __attribute__((always_inline)) {
-    const float s = T::from_bits((unsigned short)csw), z = (float)czw;
-#pragma unroll
-    for (int j = 0; j < P::WORDS; ++j) {
-      float c[8];
-      i4_codes(cw[j], c);
-      u32x4 w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = T::pack2((c[2 * e] - z) * s, (c[2 * e + 1] - z) * s);
-      if (k0 + wk + 8 * j >= a.K) w = u32x4{};
-      *reinterpret_cast<u32x4*>(lds + stage + P::BM * 128 + i4_place(wrow, wk / 8 + j)) = w;
-    }
   };
 
-  f32x4 acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{};
-
-  const int nk = (a.K + 63) / 64;
-  load_x(0, 0);
-  load_w(0);
-  make_w(0, 0);
-  auto meet = [&]() __attribute__((always_inline)) {  // what every wavefront has put into LDS, by either way, is there
-    __builtin_amdgcn_s_waitcnt(0x0070);
-    __syncthreads();
+  const int whole = end == tiles && a.K % 128 != 0 ? end - 1 : end;
+  auto meet = [&](auto left) __attribute__((always_inline)) {  // all but the `left` youngest loads are there, for every wavefront
+    constexpr int N = decltype(left)::value;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);  // (and its own reads are done)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   };
-  meet();
-  for (int kt = 0; kt < nk; ++kt) {
-    const int stage = (kt & 1) * P::STAGE, other = P::STAGE - stage;
-    const bool more = kt + 1 < nk;
-    if (more) {
-      load_x((kt + 1) * 64, other);
-      load_w((kt + 1) * 64);
+  // Weights are requested as far ahead as x, STAGES - 1 k tiles, behind the last one the last one's again: the number of loads that may
+  // still be on their way is the same at every k tile.
+  constexpr int AHEAD = STAGES - 1;
+  if (first < whole) {
+    Weights w[STAGES];
+    using S0 = std::integral_constant<int, 0>;
+    using S1 = std::integral_constant<int, 1>;
+    using S2 = std::integral_constant<int, 2>;
+    auto ask = [&](auto stage, int kt) __attribute__((always_inline)) {
+      constexpr int S = decltype(stage)::value;
+      load_x(kt, S);
+      load_w(w[S], min(kt, whole - 1));
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto step = [&](auto stage, int kt) __attribute__((always_inline)) {
+      constexpr int S = decltype(stage)::value;
+      meet(std::integral_constant<int, (AHEAD - 1) * P::ISSUED>{});
+      ask(std::integral_constant<int, (S + AHEAD) % STAGES>{}, kt + AHEAD);
+      multiply(w[S], S);
+    };
+    static_assert(STAGES == 2 || STAGES == 3, "");
+    ask(S0{}, first);
+    if constexpr (STAGES > 2) ask(S1{}, first + 1);
+    for (int kt = first;;) {  // (every way out is a break: a way round that no loop takes would be waited for)
+      step(S0{}, kt);
+      if (++kt >= whole) break;
+      step(S1{}, kt);
+      if (++kt >= whole) break;
+      if constexpr (STAGES > 2) {
+        step(S2{}, kt);
+        if (++kt >= whole) break;
+      }
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      u32x4 fx[FM], fw[FN];
-#pragma unroll
-      for (int i = 0; i < FM; ++i) fx[i] = *reinterpret_cast<const u32x4*>(lds + stage + i4_place((wm * FM + i) * 16 + lr, 4 * h + lq));
-#pragma unroll
-      for (int j = 0; j < FN; ++j) fw[j] = *reinterpret_cast<const u32x4*>(lds + stage + P::BM * 128 + i4_place((wn * FN + j) * 16 + lr, 4 * h + lq));
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma16(fw[j], fx[i], acc[i][j]);
-    }
-    if (more) make_w((kt + 1) * 64, other);
-    meet();
+  } else {
+    load_x(first, 0);  // (only the careful one)
   }
+  if (whole < end) {
+    // its rows were requested with the others; its weights are not
+    Weights w;
+    load_w_careful(w, whole);
+    meet(std::integral_constant<int, 0>{});
+    multiply(w, (whole - first) % STAGES);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // (the last loads land before the LDS is given back)
 
-  // ---- a lane holds row 16 i + lr and 4 FN adjacent columns
-  const int n = n0 + wn * 16 * FN + 4 * FN * lq;
-  float bias[4 * FN];
+  // ---- a lane holds row 16 i + lr and 4 NT adjacent columns
+  const int n = n0 + 4 * NT * lq;
+  if (n >= a.N) return;
+  if (a.parts) {
 #pragma unroll
-  for (int c = 0; c < 4 * FN; ++c) bias[c] = a.bias ? a.bias[min(n + c, a.N - 1)] : 0.f;
+    for (int i = 0; i < MT; ++i) {
+      const int m = m0 + 16 * i + lr;
+      if (m >= a.M) continue;
+      float* part = a.parts + ((int64_t)blockIdx.y * a.M + m) * a.N + n;
+      if (n + 4 * NT <= a.N) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = m0 + (wm * FM + i) * 16 + lr;
-    if (m >= a.M || n >= a.N) continue;
+        for (int j = 0; j < NT; ++j) __builtin_memcpy(part + 4 * j, &acc[i][j], 16);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4 * NT; ++c)
+          if (n + c < a.N) part[c] = acc[i][c / 4][c % 4];
+      }
+    }
+    return;
+  }
+  float bias[4 * NT];
+#pragma unroll
+  for (int c = 0; c < 4 * NT; ++c) bias[c] = a.bias ? a.bias[min(n + c, a.N - 1)] : 0.f;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int m = m0 + 16 * i + lr;
+    if (m >= a.M) continue;
     unsigned short* y = a.y + (int64_t)m * a.ldy + n;
-    unsigned int o[2 * FN];
+    unsigned int o[2 * NT];
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         o[2 * j + e] = T::pack2(acc[i][j][2 * e] + bias[4 * j + 2 * e], acc[i][j][2 * e + 1] + bias[4 * j + 2 * e + 1]);
-    if (n + 4 * FN <= a.N) {
-      __builtin_memcpy(y, o, 8 * FN);
+    if (n + 4 * NT <= a.N) {
+      __builtin_memcpy(y, o, 8 * NT);
     } else {
 #pragma unroll
-      for (int c = 0; c < 4 * FN; ++c)
+      for (int c = 0; c < 4 * NT; ++c)
         if (n + c < a.N) y[c] = (unsigned short)(o[c >> 1] >> (16 * (c & 1)));
     }
   }
@@ -192,20 +288,40 @@ __global__ __launch_bounds__(256) void i4_sum_kernel(I4Args a, int splits) {
   }
 }
 
+// How a product is done, from its sizes alone (the workspace is asked for before the call)
+struct I4Plan {
+  int dense;   // columns / 32 of the dense product's tile, or 0
+  int tall;    // 128 x 128 tiles; else 64 x 64
+  int splits;  // of K
+};
+static I4Plan i4_plan(int64_t M, int N, int K) {
+  I4Plan p = {i4_dense_tile(M, N, K), 0, 1};
+  if (p.dense || (M <= SAMFAST_I4_FEW_ROWS && N >= 16)) return p;
+  p.tall = ((M + 127) / 128) * ((N + 127) / 128) >= 256;
+  return p;
+}
+
 template <class T>
-static int launch_i4_tiled(I4Args a, hipStream_t stream) {
-  auto go = [&](auto fm, auto fn) {
-    using P = I4Tile<T, decltype(fm)::value, decltype(fn)::value>;
+static int launch_i4_tiled(I4Args a, const I4Plan& plan, hipStream_t stream) {
+  auto go = [&](auto mt, auto nt, auto waves, auto stages) {
+    using P = I4Tile<decltype(mt)::value, decltype(nt)::value, decltype(waves)::value, decltype(stages)::value>;
     a.tiles_m = (a.M + P::BM - 1) / P::BM;
     a.tiles_n = (a.N + P::BN - 1) / P::BN;
-    const dim3 grid((unsigned int)(((int64_t)a.tiles_m * a.tiles_n + 7) / 8 * 8));
-    hipLaunchKernelGGL((linear_i4_tiled_kernel<T, decltype(fm)::value, decltype(fn)::value>), grid, dim3(256), 0, stream, a);
-    return check_launch("linear_i4_tiled_kernel");
+    const dim3 grid((unsigned int)(((int64_t)a.tiles_m * a.tiles_n + 7) / 8 * 8), (unsigned int)plan.splits);
+    hipLaunchKernelGGL((linear_i4_kernel<T, decltype(mt)::value, decltype(nt)::value, decltype(waves)::value, decltype(stages)::value>), grid,
+                       dim3(64 * decltype(waves)::value), 0, stream, a);
+    if (const int rc = check_launch("linear_i4_kernel")) return rc;
+    if (!a.parts) return SAMFAST_OK;
+    hipLaunchKernelGGL(i4_sum_kernel<T>, dim3((unsigned int)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256)), dim3(256), 0, stream, a, plan.splits);
+    return check_launch("i4_sum_kernel");
   };
-  using F2 = std::integral_constant<int, 2>;
-  using F4 = std::integral_constant<int, 4>;
-  if ((int64_t)((a.M + 127) / 128) * ((a.N + 127) / 128) >= 256) return go(F4{}, F4{});
-  return go(F2{}, F2{});
+  using C1 = std::integral_constant<int, 1>;
+  using C2 = std::integral_constant<int, 2>;
+  using C3 = std::integral_constant<int, 3>;
+  using C4 = std::integral_constant<int, 4>;
+  using C8 = std::integral_constant<int, 8>;
+  if (plan.tall) return go(C8{}, C2{}, C4{}, C2{});
+  return go(C4{}, C1{}, C4{}, C3{});
 }
 
 }  // namespace samfast
@@ -213,7 +329,8 @@ static int launch_i4_tiled(I4Args a, hipStream_t stream) {
 extern "C" int64_t samfast_linear_i4_workspace(int64_t M, int N, int K) {
   using namespace samfast;
   SF_REQUIRE(M >= 0 && N > 0 && K > 0, "linear_i4_workspace: bad shape M=%lld N=%d K=%d", (long long)M, N, K);
-  return i4_dense_tile(M, N, K) ? (int64_t)N * K * 2 : 0;
+  const I4Plan plan = i4_plan(M, N, K);
+  return plan.dense ? (int64_t)N * K * 2 : plan.splits > 1 ? (int64_t)plan.splits * M * N * 4 : 0;
 }
 
 extern "C" int samfast_linear_i4(const void* x, int64_t ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros, const float* bias,
@@ -229,6 +346,9 @@ extern "C" int samfast_linear_i4(const void* x, int64_t ldx, const uint8_t* code
   SF_REQUIRE(ldx >= K && ldx % 8 == 0 && ldy >= N, "linear_i4: row strides must hold a row, that of x be a multiple of 8");
   SF_REQUIRE(aligned16(x) && (reinterpret_cast<uintptr_t>(codes) & 3u) == 0 && (reinterpret_cast<uintptr_t>(bias) & 3u) == 0,
              "linear_i4: x must be 16-byte aligned, codes and bias 4-byte");
+  const I4Plan plan = i4_plan(M, N, K);
+  SF_REQUIRE((plan.dense == 0 && plan.splits == 1) || (workspace && aligned16(workspace)),
+             "linear_i4: this shape needs a 16-byte aligned workspace (samfast_linear_i4_workspace)");
   I4Args a = {};
   a.x = reinterpret_cast<const unsigned short*>(x);
   a.codes = codes;
@@ -244,9 +364,8 @@ extern "C" int samfast_linear_i4(const void* x, int64_t ldx, const uint8_t* code
   a.group = group;
   a.div_group = i4_divider(group < K ? group : (K + 31) / 32 * 32);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int tile = i4_dense_tile(M, N, K);
-  SF_REQUIRE(tile == 0 || (workspace && aligned16(workspace)), "linear_i4: this shape needs a 16-byte aligned workspace (samfast_linear_i4_workspace)");
-  if (tile != 0 && ldy % 8 == 0 && ldy < (1 << 22) && aligned16(y)) return launch_i4_dense(a, dtype == SAMFAST_F16, tile, workspace, s);
+  if (plan.dense && ldy % 8 == 0 && ldy < (1 << 22) && aligned16(y)) return launch_i4_dense(a, dtype == SAMFAST_F16, plan.dense, workspace, s);
   if (M <= SAMFAST_I4_FEW_ROWS && N >= 16) return launch_i4_few(a, dtype == SAMFAST_F16, s);
-  return dtype == SAMFAST_F16 ? launch_i4_tiled<ElemF16>(a, s) : launch_i4_tiled<ElemBf16>(a, s);
+  if (plan.splits > 1) a.parts = reinterpret_cast<float*>(workspace);
+  return dtype == SAMFAST_F16 ? launch_i4_tiled<ElemF16>(a, plan, s) : launch_i4_tiled<ElemBf16>(a, plan, s);
 }

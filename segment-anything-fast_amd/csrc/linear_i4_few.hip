@@ -10,21 +10,6 @@
 
 namespace samfast {
 
-// words j of the lanes of quarter q: word q of the lanes of quarter j
-SF_DEVICE void i4_transpose(u32x4& w) {
-  typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
-  u32x2_t r = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false));
-  const unsigned int a0 = r[0], a2 = r[1];
-  r = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false));
-  const unsigned int a1 = r[0], a3 = r[1];
-  r = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(a0, a1, false, false));
-  w[0] = r[0];
-  w[1] = r[1];
-  r = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(a2, a3, false, false));
-  w[2] = r[0];
-  w[3] = r[1];
-}
-
 template <class T>
 struct I4Few;
 template <>
@@ -38,13 +23,11 @@ struct I4Few<ElemF16> {
   static SF_DEVICE unsigned int two(unsigned int bytes) { return __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(bytes, 512.f, HI)); }
 };
 
-// The eight codes of a word as numbers 0 to 15 of the element type, in the order of k.  As an e4m3 byte a code c is c / 512, subnormal or not, so a
-// conversion with the scale 512 makes two of them; 9 instructions for 23 with i4_codes.
+// The eight codes of a word as numbers 0 to 15 of the element type, in the order of k: 9 instructions for 23 with i4_codes
 template <class T>
 SF_DEVICE u32x4 i4_numbers(unsigned int w) {
-  const unsigned int even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
-  const unsigned int a = __builtin_amdgcn_perm(odd, even, 0x05010400u), b = __builtin_amdgcn_perm(odd, even, 0x07030602u);
-  return u32x4{I4Few<T>::template two<false>(a), I4Few<T>::template two<true>(a), I4Few<T>::template two<false>(b), I4Few<T>::template two<true>(b)};
+  const u32x2 bytes = i4_bytes(w);
+  return u32x4{I4Few<T>::template two<false>(bytes[0]), I4Few<T>::template two<true>(bytes[0]), I4Few<T>::template two<false>(bytes[1]), I4Few<T>::template two<true>(bytes[1])};
 }
 
 // MT x 16 rows, NT x 16 columns; STEPS matrix instructions (of 32 k) to a group, 4 also for longer ones.
@@ -224,8 +207,10 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
     load(next, unit(0));
     for (int n = 0; n < count; ++n) {
       const int p = unit(n), after = unit(min(n + 1, count - 1));
+      __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt 0: this wavefront's lines are in LDS
       asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
       const Weights now = next;
       hand_round(now);
       u32x4 x[2][MT][4];
@@ -235,8 +220,10 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int t = 0; t < 4; ++t) x[h][i][t] = piece(((2 * h + t / 2) * 2 * MT + 2 * i) * 1024, lr, 4 * (t & 1) + lq);
+      __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt 0: and out of it again
       asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
       request(after);
       load(next, after);
 #pragma unroll

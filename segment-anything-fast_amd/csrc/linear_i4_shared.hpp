@@ -37,6 +37,27 @@ SF_DEVICE void i4_codes(unsigned int w, float (&c)[8]) {
   }
 }
 
+// The same as bytes.  As an e4m3 number a byte c below 16 is c / 512, subnormal or not: conversions with the scale 512 give c itself.
+SF_DEVICE u32x2 i4_bytes(unsigned int w) {
+  const unsigned int even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+  return u32x2{__builtin_amdgcn_perm(odd, even, 0x05010400u), __builtin_amdgcn_perm(odd, even, 0x07030602u)};
+}
+
+// words j of the lanes of quarter q: word q of the lanes of quarter j
+SF_DEVICE void i4_transpose(u32x4& w) {
+  typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+  u32x2_t r = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false));
+  const unsigned int a0 = r[0], a2 = r[1];
+  r = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false));
+  const unsigned int a1 = r[0], a3 = r[1];
+  r = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(a0, a1, false, false));
+  w[0] = r[0];
+  w[1] = r[1];
+  r = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(a2, a3, false, false));
+  w[2] = r[0];
+  w[3] = r[1];
+}
+
 int launch_i4_few(const I4Args& a, bool f16, hipStream_t stream);  // linear_i4_few.hip: up to SAMFAST_I4_FEW_ROWS rows
 
 // linear_i4_dense.hip: the weights written out once, then the half types' product by turns.  The tile's columns / 32, 0: not this way
