@@ -39,22 +39,23 @@ SF_DEVICE u32x4 i4_weights(ElemF16, unsigned int w, float scale, float zero) {
   return o;
 }
 
-// Tiles of 16 MT rows and 16 NT WAVES columns, K 128 at a time.  The rows of x are everybody's and go through LDS, STAGES k tiles of them; the columns
-// are one wavefront's each, so that a weight is made once in the workgroup and never leaves the registers.
-template <int MT, int NT, int WAVES, int STAGES>
+// Tiles of 16 MT rows and 16 NT COLS columns, K 128 at a time.  The rows of x are everybody's and go through LDS, one k tile ahead; the columns are
+// one wavefront's each, so that a weight is made once in the workgroup and never leaves the registers.  With two SIDES as many wavefronts again take
+// every other k tile, and the sides' sums meet in LDS.  (x and weights two k tiles ahead were level: 512 x 8192 x 8192 77 / 78 us.)
+template <int MT, int NT, int COLS, int SIDES>
 struct I4Tile {
-  static constexpr int BM = 16 * MT, BN = 16 * NT * WAVES, STAGE = BM * 256;
-  static constexpr int LOADS = 4 * MT / WAVES;  // of a wavefront for a k tile of x: eight rows' lines each
-  static constexpr int ISSUED = LOADS + 2 * NT;  // with codes and scales (zeros not counted: then a few more have landed than need be)
-  static_assert(4 * MT % WAVES == 0 && STAGES * STAGE <= 160 * 1024 && (STAGES - 1) * ISSUED < 64, "");
+  static constexpr int BM = 16 * MT, BN = 16 * NT * COLS, STAGE = BM * 256, THREADS = 64 * COLS * SIDES;
+  static constexpr int LOADS = 4 * MT / COLS;  // of a wavefront for a k tile of x: eight rows' lines each
+  static_assert(4 * MT % COLS == 0 && (SIDES == 1 || SIDES == 2) && (SIDES == 1 || COLS * MT * NT * 1024 <= 2 * SIDES * STAGE) && 2 * SIDES * STAGE <= 160 * 1024, "");
 };
 
-template <class T, int MT, int NT, int WAVES, int STAGES>
-__global__ __launch_bounds__(64 * WAVES, 2) void linear_i4_kernel(I4Args a) {
-  using P = I4Tile<MT, NT, WAVES, STAGES>;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[STAGES * P::STAGE];
+template <class T, int MT, int NT, int COLS, int SIDES>
+__global__ __launch_bounds__(64 * COLS * SIDES, 2) void linear_i4_kernel(I4Args a) {
+  using P = I4Tile<MT, NT, COLS, SIDES>;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * SIDES * P::STAGE];
   const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % COLS, side = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / COLS;
+  unsigned char* mine = lds + 2 * side * P::STAGE;
 
   // neighbours on an XCD share a column of tiles, eight rows of them at a time
   const unsigned int total = (unsigned int)a.tiles_m * (unsigned int)a.tiles_n;
@@ -73,19 +74,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_i4_kernel(I4Args a) {
   int x_k[P::LOADS];
 #pragma unroll
   for (int i = 0; i < P::LOADS; ++i) {
-    const int q = wave + WAVES * i, row = 8 * (q % (2 * MT)) + (lane >> 3);
+    const int q = wave + COLS * i, row = 8 * (q % (2 * MT)) + (lane >> 3);
     x_k[i] = q / (2 * MT) * 64 + ((lane & 7) ^ ((row >> 1) & 7)) * 8;
     x_off[i] = m0 + row < a.M ? (unsigned int)row * (unsigned int)(a.ldx * 2) + 2 * x_k[i] : kOutside;
   }
   const unsigned short* xt = a.x + (int64_t)m0 * a.ldx;
   auto load_x = [&](int kt, int stage) __attribute__((always_inline)) {
-    unsigned char* to = lds + stage * P::STAGE;
+    unsigned char* to = mine + stage * P::STAGE;
 #pragma unroll
-    for (int i = 0; i < P::LOADS; ++i) piece_to_lds(xt + kt * 128, kt * 128 + x_k[i] < a.K ? x_off[i] : kOutside, to + (wave + WAVES * i) * 1024);
+    for (int i = 0; i < P::LOADS; ++i) piece_to_lds(xt + kt * 128, kt * 128 + x_k[i] < a.K ? x_off[i] : kOutside, to + (wave + COLS * i) * 1024);
   };
   auto x_piece = [&](int stage, int i, int t) __attribute__((always_inline)) {
     const int row = 16 * i + lr, c = 4 * (t & 1) + lq;
-    return *reinterpret_cast<const u32x4*>(lds + stage * P::STAGE + (t >> 1) * P::BM * 128 + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
+    return *reinterpret_cast<const u32x4*>(mine + stage * P::STAGE + (t >> 1) * P::BM * 128 + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
   };
 
   // ---- weights: row r of fragment j holds column 4 NT (r / 4) + 4 j + r % 4, so that a lane ends with 4 NT adjacent ones.  A lane has its
@@ -126,18 +127,26 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_i4_kernel(I4Args a) {
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{};
+  const bool one_group = a.group % 128 == 0;  // for a whole k tile
   auto multiply = [&](const Weights& w, int stage) __attribute__((always_inline)) {
-    u32x4 c[NT];
-    unsigned int sz[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      c[j] = w.codes[j];
-      i4_transpose(c[j]);
-      sz[j] = w.scale[j] | (a.zeros ? w.zero[j] : 8u) << 24;  // (to the top: of a byte in a register nothing has to be cleared before it is loaded)
-    }
-    u32x4 x[2][MT];
+    u32x4 x[2][MT], f[4][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) x[0][i] = x_piece(stage, i, 0);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      u32x4 c = w.codes[j];
+      i4_transpose(c);
+      const unsigned int sz = w.scale[j] | (a.zeros ? w.zero[j] : 8u) << 24;  // (to the top: of a byte in a register nothing has to be cleared before it is loaded)
+      unsigned int of[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) of[t] = sz;
+      if (!one_group) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) of[t] = (unsigned int)__builtin_amdgcn_ds_bpermute(4 * (16 * t + lr), (int)sz);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) f[t][j] = i4_weights(T{}, c[t], T::from_bits((unsigned short)of[t]), (float)(of[t] >> 24));
+    }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (t < 3) {
@@ -145,68 +154,67 @@ __global__ __launch_bounds__(64 * WAVES, 2) void linear_i4_kernel(I4Args a) {
         for (int i = 0; i < MT; ++i) x[(t + 1) & 1][i] = x_piece(stage, i, t + 1);
       }
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const unsigned int g = (unsigned int)__builtin_amdgcn_ds_bpermute(4 * (16 * t + lr), (int)sz[j]);
-        const u32x4 f = i4_weights(T{}, c[j][t], T::from_bits((unsigned short)g), (float)(g >> 24));
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i][j] = T::mfma16(f, x[t & 1][i], acc[i][j]);
-      }
+        for (int i = 0; i < MT; ++i) acc[i][j] = T::mfma16(f[t][j], x[t & 1][i], acc[i][j]);
     }
   };
 
   const int whole = end == tiles && a.K % 128 != 0 ? end - 1 : end;
-  auto meet = [&](auto left) __attribute__((always_inline)) {  // all but the `left` youngest loads are there, for every wavefront
-    constexpr int N = decltype(left)::value;
+  auto meet = [&]() __attribute__((always_inline)) {  // all loads are there, for every wavefront, and all reads done
     __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);  // (and its own reads are done)
+    __builtin_amdgcn_s_waitcnt(0x0070);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  // Weights are requested as far ahead as x, STAGES - 1 k tiles, behind the last one the last one's again: the number of loads that may
-  // still be on their way is the same at every k tile.
-  constexpr int AHEAD = STAGES - 1;
+  Weights w[2];
+  auto ask = [&](auto stage, int kt) __attribute__((always_inline)) {  // (behind the last: x outside, or another workgroup's; the last weights again)
+    constexpr int S = decltype(stage)::value;
+    load_x(kt, S);
+    if (first < whole) load_w(w[S], min(kt, whole - 1));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  int kt = first + side;
+  ask(S0{}, kt);
   if (first < whole) {
-    Weights w[STAGES];
-    using S0 = std::integral_constant<int, 0>;
-    using S1 = std::integral_constant<int, 1>;
-    using S2 = std::integral_constant<int, 2>;
-    auto ask = [&](auto stage, int kt) __attribute__((always_inline)) {
-      constexpr int S = decltype(stage)::value;
-      load_x(kt, S);
-      load_w(w[S], min(kt, whole - 1));
-      __builtin_amdgcn_sched_barrier(0);
+    auto step = [&](auto stage, auto other) __attribute__((always_inline)) {
+      meet();
+      ask(other, kt + SIDES);
+      if (SIDES == 1 || kt < whole) multiply(w[decltype(stage)::value], decltype(stage)::value);
+      kt += SIDES;
     };
-    auto step = [&](auto stage, int kt) __attribute__((always_inline)) {
-      constexpr int S = decltype(stage)::value;
-      meet(std::integral_constant<int, (AHEAD - 1) * P::ISSUED>{});
-      ask(std::integral_constant<int, (S + AHEAD) % STAGES>{}, kt + AHEAD);
-      multiply(w[S], S);
-    };
-    static_assert(STAGES == 2 || STAGES == 3, "");
-    ask(S0{}, first);
-    if constexpr (STAGES > 2) ask(S1{}, first + 1);
-    for (int kt = first;;) {  // (every way out is a break: a way round that no loop takes would be waited for)
-      step(S0{}, kt);
-      if (++kt >= whole) break;
-      step(S1{}, kt);
-      if (++kt >= whole) break;
-      if constexpr (STAGES > 2) {
-        step(S2{}, kt);
-        if (++kt >= whole) break;
-      }
+    for (;;) {
+      step(S0{}, S1{});
+      if (kt - side >= whole) break;
+      step(S1{}, S0{});
+      if (kt - side >= whole) break;
     }
-  } else {
-    load_x(first, 0);  // (only the careful one)
   }
-  if (whole < end) {
-    // its rows were requested with the others; its weights are not
-    Weights w;
-    load_w_careful(w, whole);
-    meet(std::integral_constant<int, 0>{});
-    multiply(w, (whole - first) % STAGES);
+  meet();
+  if (whole < end && (whole - first) % SIDES == side) {  // its rows were requested with the others
+    Weights last;
+    load_w_careful(last, whole);
+    multiply(last, (whole - first) / SIDES % 2);
   }
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // (the last loads land before the LDS is given back)
+  if constexpr (SIDES == 2) {
+    meet();
+    f32x4* sums = reinterpret_cast<f32x4*>(lds) + wave * MT * NT * 64 + lane;
+    if (side == 1) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sums[(i * NT + j) * 64] = acc[i][j];
+    }
+    meet();
+    if (side == 1) return;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] += sums[(i * NT + j) * 64];
+  }
 
   // ---- a lane holds row 16 i + lr and 4 NT adjacent columns
   const int n = n0 + 4 * NT * lq;
@@ -288,28 +296,54 @@ __global__ __launch_bounds__(256) void i4_sum_kernel(I4Args a, int splits) {
   }
 }
 
-// How a product is done, from its sizes alone (the workspace is asked for before the call)
+// How a product is done, from its sizes alone (the workspace is asked for before the call): what takes least by these estimates in us, which lie within
+// a fifth of the times measured.
+//   tiles: 4 + a k tile's time x k tiles x tiles to a CU, alone on it / not; + 3 and the sums' bytes at 6 TB/s where K is split.  Measured, 32 x 64 / 64 x 64 /
+//     128 x 128 tiles: 128 x 1280 -> 3840 7.0 / 8.5 / 12, 333 x 1000 -> 1003 7.5 / 8.8 / 12, 256 x 4096 -> 4096 23.5 / 20.9 / 23 (K split), 512 x 4096 -> 4096
+//     - / 31.2 / 33, 1024 x 1280 -> 3840 - / 22.3 / 18.0, 8000 x 4096 -> 3001 - / 262 / 197; K whole / in four: 64 x 4096 -> 4096 20 / 11.9, 64 x 8192 -> 8192 35 / 20.9,
+//     256 x 4096 -> 4096 20.9 / 24.
+//   dense (linear_i4_dense.hip): by its own estimate.  tiles / dense: 4096 x 1280 -> 5120 58 / 50, 16384 x 1280 -> 5120 204 / 160, but 4096 x 1280 -> 1280 25 / 33,
+//     1024 x 8192 -> 8192 135 / 153.
+// Up to SAMFAST_I4_FEW_ROWS rows linear_i4_few.hip: 24 x 4096 -> 4096 7.7, tiles 15.
 struct I4Plan {
   int dense;   // columns / 32 of the dense product's tile, or 0
-  int tall;    // 128 x 128 tiles; else 64 x 64
+  int tile;    // 32 x 64, 64 x 64, 128 x 128
   int splits;  // of K
 };
 static I4Plan i4_plan(int64_t M, int N, int K) {
-  I4Plan p = {i4_dense_tile(M, N, K), 0, 1};
-  if (p.dense || (M <= SAMFAST_I4_FEW_ROWS && N >= 16)) return p;
-  p.tall = ((M + 127) / 128) * ((N + 127) / 128) >= 256;
+  I4Plan p = {0, 0, 1};
+  if (M <= SAMFAST_I4_FEW_ROWS && N >= 16) return p;
+  static const struct { int rows, cols, sides; double alone, beside; } kTiles[3] = {{32, 64, 2, 0.35, 0.30}, {64, 64, 2, 0.52, 0.42}, {128, 128, 1, 1.25, 1.0}};
+  const int k_tiles = (K + 127) / 128;
+  double least = 0.0;
+  for (int t = 0; t < 3; ++t)
+    for (int splits : {1, 2, 3, 4, 6, 8}) {
+      const int sides = kTiles[t].sides;
+      if (splits > 1 && k_tiles < 2 * splits) break;
+      const int each = ((k_tiles + splits - 1) / splits + sides - 1) / sides * sides;
+      const double blocks = (double)((M + kTiles[t].rows - 1) / kTiles[t].rows) * ((N + kTiles[t].cols - 1) / kTiles[t].cols) * splits / 256.0;
+      const double time = 4.0 + each * (blocks <= 1.0 ? kTiles[t].alone : blocks <= 4.0 ? (double)(int)(blocks + 0.999) * kTiles[t].beside : blocks * kTiles[t].beside) +
+                          (splits > 1 ? 3.0 + 8.0 * splits * (double)M * N / 6e6 : 0.0);
+      if (least == 0.0 || time < least) {
+        least = time;
+        p = I4Plan{0, t, splits};
+      }
+    }
+  double dense = 0.0;
+  const int columns = i4_dense_tile(M, N, K, &dense);
+  if (columns && dense < least) p = I4Plan{columns, 0, 1};
   return p;
 }
 
 template <class T>
 static int launch_i4_tiled(I4Args a, const I4Plan& plan, hipStream_t stream) {
-  auto go = [&](auto mt, auto nt, auto waves, auto stages) {
-    using P = I4Tile<decltype(mt)::value, decltype(nt)::value, decltype(waves)::value, decltype(stages)::value>;
+  auto go = [&](auto mt, auto nt, auto cols, auto sides) {
+    using P = I4Tile<decltype(mt)::value, decltype(nt)::value, decltype(cols)::value, decltype(sides)::value>;
     a.tiles_m = (a.M + P::BM - 1) / P::BM;
     a.tiles_n = (a.N + P::BN - 1) / P::BN;
     const dim3 grid((unsigned int)(((int64_t)a.tiles_m * a.tiles_n + 7) / 8 * 8), (unsigned int)plan.splits);
-    hipLaunchKernelGGL((linear_i4_kernel<T, decltype(mt)::value, decltype(nt)::value, decltype(waves)::value, decltype(stages)::value>), grid,
-                       dim3(64 * decltype(waves)::value), 0, stream, a);
+    hipLaunchKernelGGL((linear_i4_kernel<T, decltype(mt)::value, decltype(nt)::value, decltype(cols)::value, decltype(sides)::value>), grid,
+                       dim3(P::THREADS), 0, stream, a);
     if (const int rc = check_launch("linear_i4_kernel")) return rc;
     if (!a.parts) return SAMFAST_OK;
     hipLaunchKernelGGL(i4_sum_kernel<T>, dim3((unsigned int)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256)), dim3(256), 0, stream, a, plan.splits);
@@ -317,11 +351,11 @@ static int launch_i4_tiled(I4Args a, const I4Plan& plan, hipStream_t stream) {
   };
   using C1 = std::integral_constant<int, 1>;
   using C2 = std::integral_constant<int, 2>;
-  using C3 = std::integral_constant<int, 3>;
   using C4 = std::integral_constant<int, 4>;
   using C8 = std::integral_constant<int, 8>;
-  if (plan.tall) return go(C8{}, C2{}, C4{}, C2{});
-  return go(C4{}, C1{}, C4{}, C3{});
+  if (plan.tile == 0) return go(C2{}, C1{}, C4{}, C2{});
+  if (plan.tile == 1) return go(C4{}, C1{}, C4{}, C2{});
+  return go(C8{}, C1{}, C8{}, C1{});
 }
 
 }  // namespace samfast

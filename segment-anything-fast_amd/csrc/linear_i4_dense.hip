@@ -22,10 +22,15 @@ __global__ __launch_bounds__(256) void i4_weights_kernel(I4Args a, unsigned shor
   reinterpret_cast<u32x4*>(w)[i] = o;
 }
 
-int i4_dense_tile(int64_t M, int N, int K) {
-  if (K % 64 != 0 || K < 320 || N % 8 != 0 || M < 512) return 0;
+// The time: a launch, the weights read and written, and pp_choose's cost, a unit of which takes 0.085 us where the GPU is nearly idle and 0.115 where it is
+// busy throughout (power).  2048 x 4096 -> 4096 72 us, 4096 x 1280 -> 5120 50, 65536 x 1280 -> 3840 479, 1024 x 8192 -> 8192 153.
+int i4_dense_tile(int64_t M, int N, int K, double* time) {
+  if (K % 64 != 0 || K < 320 || N % 8 != 0 || M < 256) return 0;
   const PPChoice c = pp_choose(M, N, K / 64, false, 8.1);
-  return c.tn != 0 && c.used >= 0.5 ? c.tn : 0;
+  if (c.tn == 0) return 0;
+  const double fragments = c.tn == 10 ? 12.5 : c.tn == 8 ? 10.0 : 8.1;
+  *time = 4.0 + 2.5 * (double)N * K / 5e6 + (0.085 + 0.03 * c.used) * (double)c.rounds * fragments * (K / 64 + 8);
+  return c.tn;
 }
 
 template <class T, class E>

@@ -60,8 +60,9 @@ SF_DEVICE void i4_transpose(u32x4& w) {
 
 int launch_i4_few(const I4Args& a, bool f16, hipStream_t stream);  // linear_i4_few.hip: up to SAMFAST_I4_FEW_ROWS rows
 
-// linear_i4_dense.hip: the weights written out once, then the half types' product by turns.  The tile's columns / 32, 0: not this way
-int i4_dense_tile(int64_t M, int N, int K);
+// linear_i4_dense.hip: the weights written out once, then the half types' product by turns.  The tile's columns / 32 and about how many us it
+// takes; 0: not this way
+int i4_dense_tile(int64_t M, int N, int K, double* time);
 int launch_i4_dense(const I4Args& a, bool f16, int tile, void* weights, hipStream_t stream);
 
 }  // namespace samfast
