@@ -684,6 +684,26 @@ def _require_here(name: str, *tensors: Optional[torch.Tensor]) -> None:
             raise RuntimeError(f"samfast: {name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """First byte and the byte behind the last that a tensor's elements lie in."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride()
+
+
+def _check_out(name: str, out: torch.Tensor, own: Sequence[torch.Tensor], others: Sequence[Optional[torch.Tensor]]) -> None:
+    """`out` is one of `own`, or lies apart from all of `own` and `others`, and no two of its elements share memory."""
+    if any(_same_view(out, t) for t in own):
+        return
+    a, b = _span(out)
+    clash = any(t is not None and max(a, _span(t)[0]) < min(b, _span(t)[1]) for t in (*own, *others))
+    if clash or torch._debug_has_internal_overlap(out) == 1:
+        raise RuntimeError(f"samfast: {name}'s out overlaps itself or an input in another way than being one")
+
+
 def linear_i4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
               bias: Optional[torch.Tensor] = None, *, group_size: int) -> torch.Tensor:
     """Linear with 4-bit weights on half-type rows x (..., K): y = x w^T + bias with w[n, k] = (code[n, k] - zeros[g, n]) * scales[g, n],
@@ -749,8 +769,8 @@ def norm_residual(x: torch.Tensor, residual: torch.Tensor, *, gate: Optional[tor
         total = residual_scale * residual + branch_scale * gate * post(x),   normed = pre(total)
     over the last axis of half-type rows x (..., K <= 32768).  post and pre: (gamma, beta or None, eps) of a LayerNorm, or with `rms` of an RMS
     norm, or None to leave it out (normed is then None).  residual: x's shape, x's dtype or fp32; total has its type.  gate: (K), or (G, K) with a
-    row for each of G equal runs of x's rows.  fp32 inside; pre sees the total before it is rounded.  `out`: where total goes, which may be the
-    residual.  Returns (total, normed)."""
+    row for each of G equal runs of x's rows.  fp32 inside; pre sees the total before it is rounded.  `out`: where total goes: the
+    residual itself (or x, of the same type), or memory of its own.  Returns (total, normed)."""
     if out is None and _launch_log is None:
         both = (_lib._host or _lib.host()).norm_residual(x, residual, gate, post, pre, rms, branch_scale, residual_scale)
         if both is not None:
@@ -777,6 +797,8 @@ def norm_residual(x: torch.Tensor, residual: torch.Tensor, *, gate: Optional[tor
         res = res.contiguous()
     if out is not None and (out.shape != x.shape or out.dtype != residual.dtype or not out.is_contiguous()):
         raise RuntimeError("samfast: out must be a contiguous tensor of the residual's shape and dtype")
+    if out is not None:
+        _check_out("norm_residual", out, (residual, x), (gate, post_gamma, post_beta, pre_gamma, pre_beta))
     total = torch.empty(x.shape, dtype=residual.dtype, device=x.device) if out is None else out
     normed = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre is not None else None
     ptr = lambda t: t.data_ptr() if t is not None else None
@@ -797,7 +819,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     types.  positions int64, (B, T) or (T,); frequencies fp64 (pairs,), radians a position.  For a grid positions (..., T, axes) and
     frequencies (axes, pairs).  Axis after axis, 2 * pairs channels of the head are turned: pairs of neighbours (`interleaved`), or of a channel
     and its like half of the axis's channels on; channels behind the last axis's are copied.  `scale` multiplies what is turned.  Angles are made in 64
-    bits.  Returns (q', k') in q's and k's shapes, laid out token-major (k' is None where k is), or in `out`, which may be (q, k)."""
+    bits.  Returns (q', k') in q's and k's shapes, laid out token-major (k' is None where k is), or in `out`, whose tensors are q and k themselves or memory of their own."""
     if out is None and _launch_log is None:
         both = (_lib._host or _lib.host()).rotary(q, k, positions, frequencies, interleaved, scale)
         if both is not None:
@@ -825,6 +847,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         for t, o in zip(tensors, outs):
             if o is None or o.shape != t.shape or o.dtype != t.dtype:
                 raise RuntimeError("samfast: out must hold tensors of q's and k's shapes and dtype")
+        for i, (t, o) in enumerate(zip(tensors, outs)):
+            _check_out("rotary", o, (t,), (*tensors, positions, frequencies, *outs[:i], *outs[i + 1:]))
     strides = []
     for t, o in zip(tensors, outs):
         strides += [*_bnhd_strides(t), *_bnhd_strides(o)]

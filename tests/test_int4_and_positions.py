@@ -1,0 +1,76 @@
+"""The 4-bit weight quantiser, the module that holds it, and rotary frequencies, on the CPU."""
+
+import math
+
+import pytest
+import torch
+
+
+@pytest.mark.parametrize("N,K,group", [(3, 8, 32), (5, 96, 32), (4, 200, 64), (7, 256, 256), (2, 1000, 128)])
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_codes_are_the_nearest_to_the_weights(N, K, group, zero_points, dtype):
+    from samfast_amd import quant4
+    g = torch.Generator().manual_seed(N + K)
+    w = (torch.randn((N, K), generator=g) * 0.02 + 0.005).to(dtype)
+    w[0, : min(group, K)] = 0
+    codes, scales, zeros = quant4.quantize_weight_int4(w, group, zero_points)
+    groups = -(-K // group)
+    assert codes.shape == (N, K // 2) and codes.dtype == torch.uint8 and scales.shape == (groups, N)
+    assert scales.dtype == (torch.bfloat16 if dtype == torch.float32 else dtype)
+    assert (zeros is None) == (not zero_points)
+    back = quant4.dequantize_weight_int4(codes, scales, zeros, group)
+    step = scales.float().t()[:, torch.arange(K) // group]
+    # half a step; a scale rounded down leaves the extreme value up to 7.5 (15 with zero points) roundings of it, 2^-8 each at most, outside, and
+    # a zero point is off by half a step, which the clamp at an end then adds
+    slack = (0.5 + 15 * 2.0 ** -8 + (0.5 if zero_points else 0.0)) * step
+    assert ((back - w.float()).abs() <= slack + 1e-7).all()
+    assert (back[0, : min(group, K)] == 0).all()
+    # each even input in the lower half of its byte
+    c = ((w.float()[-1, :2] / step[-1, :2]).round() + (8 if zeros is None else zeros[0, -1].float())).clamp(0, 15)
+    assert int(codes[-1, 0]) == int(c[0]) + 16 * int(c[1])
+
+
+def test_the_quantiser_refuses():
+    from samfast_amd import quant4
+    for weight, group in [(torch.zeros(4, 12), 32), (torch.zeros(4, 16), 48), (torch.zeros(4, 16), 0), (torch.zeros(16), 32), (torch.zeros(4, 16, dtype=torch.int8), 32), (torch.zeros(0, 16), 32)]:
+        with pytest.raises(ValueError):
+            quant4.quantize_weight_int4(weight, group)
+
+
+def test_module_state_and_swap():
+    from samfast_amd import Int4Linear, apply_int4_weights
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(torch.nn.Linear(64, 40), torch.nn.Sequential(torch.nn.ReLU(), torch.nn.Linear(40, 24, bias=False)), torch.nn.Linear(24, 8))
+    bias, weight = model[0].bias.detach().clone(), model[0].weight.detach().clone()
+    apply_int4_weights(model, filter_fn=lambda m, fqn: fqn != "2", group_size=32, zero_points=True)
+    assert isinstance(model[0], Int4Linear) and isinstance(model[1][1], Int4Linear) and type(model[2]) is torch.nn.Linear
+    assert model[1][1].bias is None and "groups of 32" in repr(model[0])
+    model.to(torch.float16)
+    assert torch.equal(model[0].bias, bias) and model[0].scales.dtype == torch.float16 and model[0].codes.dtype == torch.uint8
+    assert (model[0].weight - weight).abs().max() < 0.05 * weight.abs().max() + 0.02
+    other = torch.nn.Sequential(torch.nn.Linear(64, 40), torch.nn.Sequential(torch.nn.ReLU(), torch.nn.Linear(40, 24, bias=False)), torch.nn.Linear(24, 8))
+    apply_int4_weights(other, filter_fn=lambda m, fqn: fqn != "2", group_size=32, zero_points=True)
+    other.to(torch.float16).load_state_dict(model.state_dict())
+    assert torch.equal(other[0].weight, model[0].weight) and torch.equal(other[0].bias, bias)
+    state = {k: v for k, v in model[0].state_dict().items() if k != "bias_bits"}
+    other[0].load_state_dict({**state, "bias": bias + 1})
+    assert torch.equal(other[0].bias, bias + 1)
+    with pytest.raises(RuntimeError, match="samfast"):
+        model[0](torch.zeros(2, 64, dtype=torch.float16))  # no CPU route
+
+
+def test_frequencies_and_grid():
+    from samfast_amd import grid_positions, rotary_frequencies
+    f = rotary_frequencies(64)
+    assert f.dtype == torch.float64 and f[0] == 1 and abs(float(f[32]) - 0.01) < 1e-15
+    assert torch.equal(rotary_frequencies(64, scaling="linear", factor=8.0), f / 8)
+    b = rotary_frequencies(64, scaling="bands", factor=8.0, trained_length=4096)
+    turns = 4096 * f / (2 * math.pi)
+    assert torch.equal(b[turns >= 32], f[turns >= 32]) and torch.allclose(b[turns <= 1], f[turns <= 1] / 8, rtol=1e-15)
+    between = (turns > 1) & (turns < 32)
+    assert between.any() and (b[between] < f[between]).all() and (b[between] > f[between] / 8).all() and (b[1:] < b[:-1]).all()
+    for bad in (dict(pairs=0), dict(pairs=4, scaling="ntk"), dict(pairs=4, factor=0.0), dict(pairs=4, slow_turns=32.0), dict(pairs=4, base=-1.0)):
+        with pytest.raises(ValueError):
+            rotary_frequencies(**bad)
+    assert grid_positions(2, 3).tolist() == [[0, 0], [0, 1], [0, 2], [1, 0], [1, 1], [1, 2]]
