@@ -43,7 +43,7 @@ constexpr int kI4FewWaves = 8;
 template <class T, int MT, int NT, int STEPS>
 __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args a) {
   constexpr int GROUPS = 4 / STEPS;  // of 128 k
-  constexpr int XBYTES = MT * 16 * 512, OWN = XBYTES + 1024;
+  constexpr int XBYTES = MT * 16 * 512, OWN = XBYTES + 2048;
   static_assert(MT * NT * 1024 <= OWN && 2 * GROUPS * 4 * NT <= 64, "the sums fit into what the loads used, the scales into 64 lanes");
   __shared__ __attribute__((aligned(16))) unsigned char lds[kI4FewWaves * OWN];
   const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
@@ -104,7 +104,12 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
     if (a.zeros) __builtin_memcpy(&w.zeros, a.zeros + at, 4);
   };
   auto hand_round = [&](const Weights& w) __attribute__((always_inline)) {
-    *reinterpret_cast<u32x4*>(mine + XBYTES + lane * 16) = u32x4{w.scales[0], w.scales[1], w.zeros, 0u};
+    f32x4 s = {T::lo(w.scales[0]), T::hi(w.scales[0]), T::lo(w.scales[1]), T::hi(w.scales[1])}, sz;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sz[e] = -s[e] * (float)((w.zeros >> (8 * e)) & 255u);  // (exact)
+    f32x4* to = reinterpret_cast<f32x4*>(mine + XBYTES) + lane;
+    to[0] = s;
+    to[64] = sz;
   };
   auto load = [&](Weights& w, int p) __attribute__((always_inline)) {
 #pragma unroll
@@ -115,9 +120,9 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
     load_scales(w, 8 * p);
   };
   f32x4 acc[MT][NT];
-  // The products of 128 k, the h-th of those whose scales were handed round.  SIMPLE: code - zero is made before it is multiplied, with the lane's own column's zero; else the codes are, and
+  // The products of 128 k, the h-th of those whose scales, and these times the zeros, were handed round.  SIMPLE: code - zero is made before it is multiplied, with the lane's own column's zero; else the codes are, and
   // the zero times the group's sum of x, which all columns share, is taken off.
-  auto multiply = [&](const u32x4 (&cw)[NT], const u32x4 (&x)[MT][4], int h, int seg, auto simple) __attribute__((always_inline)) {
+  auto multiply = [&](const u32x4 (&cw)[NT], const u32x4 (&x)[MT][4], int h, int seg, auto simple, unsigned int zeros = 0) __attribute__((always_inline)) {
     constexpr bool SIMPLE = decltype(simple)::value;
     f32x4 sum[GROUPS][MT];
     if constexpr (!SIMPLE) {
@@ -141,10 +146,10 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
         f32x4 part[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) part[i] = f32x4{};
-        const u32x4 sz = *reinterpret_cast<const u32x4*>(mine + XBYTES + ((h * GROUPS + g) * Q + 4 * j + lq) * 16);
-        const unsigned int zw = sz[2];
+        const int from = (h * GROUPS + g) * Q + 4 * j;  // the lane that had the first four columns
+        const f32x4 s = reinterpret_cast<const f32x4*>(mine + XBYTES)[from + lq];
         float z = 0.f;
-        if constexpr (SIMPLE) z = (float)((__shfl(zw, (lr >> 2) * 16, 64) >> (8 * (lr & 3))) & 255u);
+        if constexpr (SIMPLE) z = (float)((__shfl(zeros, from + (lr >> 2), 64) >> (8 * (lr & 3))) & 255u);
 #pragma unroll
         for (int t = g * STEPS; t < (g + 1) * STEPS; ++t) {
           u32x4 w;
@@ -159,12 +164,16 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
 #pragma unroll
           for (int i = 0; i < MT; ++i) part[i] = T::mfma16(w, x[i][t], part[i]);
         }
-        const float s[4] = {T::lo(sz[0]), T::hi(sz[0]), T::lo(sz[1]), T::hi(sz[1])};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float zero = (float)((zw >> (8 * e)) & 255u);
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int i = 0; i < MT; ++i) acc[i][j][e] = fmaf(SIMPLE ? part[i][e] : fmaf(-zero, sum[g][i][e], part[i][e]), s[e], acc[i][j][e]);
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(part[i][e], s[e], acc[i][j][e]);
+        if constexpr (!SIMPLE) {
+          const f32x4 sz = reinterpret_cast<const f32x4*>(mine + XBYTES)[64 + from + lq];
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[g][i][e], sz[e], acc[i][j][e]);
         }
       }
     }
@@ -197,7 +206,7 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
         if (m0 + 16 * i + lr < a.M && seg * 128 + 32 * t + 8 * lq < a.K)
           x[i][t] = *reinterpret_cast<const u32x4*>(rows + (int64_t)(16 * i + lr) * (2 * a.ldx) + seg * 256 + 64 * t + 16 * lq);
       }
-    multiply(w.codes[0], x, 0, seg, std::true_type{});
+    multiply(w.codes[0], x, 0, seg, std::true_type{}, w.zeros);
   };
 
   clear();
@@ -206,7 +215,6 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
     request(unit(0));
     load(next, unit(0));
     for (int n = 0; n < count; ++n) {
-      const int p = unit(n), after = unit(min(n + 1, count - 1));
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt 0: this wavefront's lines are in LDS
       asm volatile("" ::: "memory");
@@ -224,13 +232,14 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt 0: and out of it again
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-      request(after);
-      load(next, after);
+      if (n + 1 < count) {
+        request(unit(n + 1));
+        load(next, unit(n + 1));
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) multiply(now.codes[h], x[h], h, 2 * p + h, std::false_type{});
+      for (int h = 0; h < 2; ++h) multiply(now.codes[h], x[h], h, 2 * unit(n) + h, std::false_type{});
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // (the last request has landed before the LDS is used for something else)
-    asm volatile("" ::: "memory");
   }
   // An infinity in a row or a scale, or sums that overflow before the zero is taken off, end as a NaN or an infinity here; the simple
   // way then gives what the formula does.
