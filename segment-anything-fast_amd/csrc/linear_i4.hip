@@ -169,10 +169,10 @@ __global__ __launch_bounds__(64 * COLS * SIDES, 2) void linear_i4_kernel(I4Args 
     __builtin_amdgcn_sched_barrier(0);
   };
   Weights w[2];
-  auto ask = [&](auto stage, int kt) __attribute__((always_inline)) {  // (behind the last: x outside, or another workgroup's; the last weights again)
+  auto ask = [&](auto stage, int kt) __attribute__((always_inline)) {
     constexpr int S = decltype(stage)::value;
-    load_x(kt, S);
-    if (first < whole) load_w(w[S], min(kt, whole - 1));
+    if (kt < end) load_x(kt, S);
+    if (kt < whole) load_w(w[S], kt);
     __builtin_amdgcn_sched_barrier(0);
   };
   using S0 = std::integral_constant<int, 0>;

@@ -22,6 +22,7 @@ struct NormResidualArgs {
   int64_t M, ldx, ld_res, group;  // rows that share a gate row
   int K;
   int halves, rows;          // of a workgroup: halves of wavefronts to a row, rows
+  int in_place;
   int rms;
   float eps_post, eps_pre, branch_scale, residual_scale, inv_K;
 };
@@ -93,7 +94,8 @@ SF_DEVICE float half_sum(float v) {  // over 32 lanes: wave_reduce without its l
 // (of 8: 65536 x 1280 238 us for 150).  What was behind that, all of it with fewer rows in flight: two rows to a thread, which then
 // share the norms' weights, 43008 x 2048 131 us for 133, but onto fp32, 21504 x 2048, 113 for 101; threads that go on to other rows with the weights kept in
 // registers, 65536 x 1280 143-180, 5003 x 8192 onto fp32 110-130.  The weights come out of the caches.
-template <class T, class R, int NCH>
+// WHOLE: K is a multiple of the pieces.
+template <class T, class R, int NCH, bool WHOLE>
 __global__ __launch_bounds__(1024) void norm_residual_kernel(NormResidualArgs a) {
   constexpr int E = 8;
   typedef Piece<unsigned short, E> P;
@@ -104,7 +106,12 @@ __global__ __launch_bounds__(1024) void norm_residual_kernel(NormResidualArgs a)
   const bool idle = half >= a.rows * a.halves || row >= a.M;  // (it meets the others at the barriers)
   const int threads = 32 * a.halves, K = idle ? 0 : a.K;
   const int first = ((int)threadIdx.x - mine * threads) * E;
-  auto at = [&](int i) __attribute__((always_inline)) { return first + i * threads * E; };
+  // Where piece i lies.  One that would end behind its row lies over the one before it, so that it is whole too (one value after the other, 44058 x 1999 took 245 us for 167); the
+  // values that belong to that one, below owned(i), are not summed.
+  auto owned = [&](int i) __attribute__((always_inline)) { return first + i * threads * E; };
+  auto at = [&](int i) __attribute__((always_inline)) { return !WHOLE && K >= E && owned(i) < K ? min(owned(i), K - E) : owned(i); };
+  auto counts = [&](int i, int e) __attribute__((always_inline)) { return WHOLE || at(i) + e >= owned(i); };
+  auto length = [&](int i) __attribute__((always_inline)) { return WHOLE ? E : K - at(i); };
 
   // everything is requested before anything is waited for, if there are registers for it
   constexpr bool AHEAD = NCH <= 2;
@@ -116,8 +123,8 @@ __global__ __launch_bounds__(1024) void norm_residual_kernel(NormResidualArgs a)
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     if (at(i) < K) {
-      xw[i].load(a.x + row * a.ldx + at(i), K - at(i));
-      rw[i].load(reinterpret_cast<const R*>(a.residual) + row * a.ld_res + at(i), K - at(i));
+      xw[i].load(a.x + row * a.ldx + at(i), length(i));
+      rw[i].load(reinterpret_cast<const R*>(a.residual) + row * a.ld_res + at(i), length(i));
     } else {
       xw[i] = {};
       rw[i] = {};
@@ -128,12 +135,16 @@ __global__ __launch_bounds__(1024) void norm_residual_kernel(NormResidualArgs a)
     for (int j = 0; j < 5; ++j)
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
-        if (from[j] && at(i) < K) ahead[j][i].load(from[j] + at(i), K - at(i));
+        if (from[j] && at(i) < K) ahead[j][i].load(from[j] + at(i), length(i));
+  }
+  if (!WHOLE && a.in_place) {  // two threads read some of a row's values: before either of them writes
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
   }
   auto weights = [&](int j, int i) __attribute__((always_inline)) {
     if constexpr (AHEAD) return ahead[j][i];
     P p;
-    p.load(from[j] + at(i), K - at(i));
+    p.load(from[j] + at(i), length(i));
     return p;
   };
 
@@ -153,18 +164,18 @@ __global__ __launch_bounds__(1024) void norm_residual_kernel(NormResidualArgs a)
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += f[i][e];
+        for (int e = 0; e < E; ++e) s += counts(i, e) ? f[i][e] : 0.f;
       const float mean = sum(s) * a.inv_K;
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[i][e] = at(i) + e < K ? f[i][e] - mean : 0.f;
+        for (int e = 0; e < E; ++e) f[i][e] = at(i) + (WHOLE ? 0 : e) < K ? f[i][e] - mean : 0.f;
     }
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
-      for (int e = 0; e < E; ++e) q = fmaf(f[i][e], f[i][e], q);
+      for (int e = 0; e < E; ++e) q = counts(i, e) ? fmaf(f[i][e], f[i][e], q) : q;
     const float scale = 1.0f / sqrtf(fmaf(sum(q), a.inv_K, eps));
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -196,11 +207,11 @@ __global__ __launch_bounds__(1024) void norm_residual_kernel(NormResidualArgs a)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       f[i][e] = fmaf(a.residual_scale, rw[i].template get<T>(e), a.branch_scale * f[i][e]);
-      if (at(i) + e >= K) f[i][e] = 0.f;
+      if (!WHOLE && at(i) + e >= K) f[i][e] = 0.f;
     }
     Piece<R, E> o;
     o.template put<T>(f[i]);
-    o.store(reinterpret_cast<R*>(a.total) + row * K + at(i), K - at(i));
+    o.store(reinterpret_cast<R*>(a.total) + row * K + at(i), length(i));
   }
   if (!a.normed) return;
   norm(3, a.eps_pre);
@@ -209,7 +220,7 @@ __global__ __launch_bounds__(1024) void norm_residual_kernel(NormResidualArgs a)
     if (at(i) >= K) continue;
     P o;
     o.template put<T>(f[i]);
-    o.store(a.normed + row * K + at(i), K - at(i));
+    o.store(a.normed + row * K + at(i), length(i));
   }
 }
 
@@ -220,17 +231,18 @@ static int launch_norm_residual(NormResidualArgs a, hipStream_t stream) {
     a.halves = (a.K + 256 * NCH - 1) / (256 * NCH);
     a.rows = a.halves % 2 == 1 && a.halves <= 15 ? 2 : 1;
     const dim3 grid((unsigned int)((a.M + a.rows - 1) / a.rows)), block((a.rows * a.halves + 1) / 2 * 64);
-    hipLaunchKernelGGL((norm_residual_kernel<T, R, NCH>), grid, block, 0, stream, a);
+    if (a.K % 8 == 0) hipLaunchKernelGGL((norm_residual_kernel<T, R, NCH, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((norm_residual_kernel<T, R, NCH, false>), grid, block, 0, stream, a);
     return check_launch("norm_residual_kernel");
   };
   using N1 = std::integral_constant<int, 1>;
   using N2 = std::integral_constant<int, 2>;
   using N4 = std::integral_constant<int, 4>;
   if (a.K > 16384) return go(N4{});
-  // One piece to a thread / two, us at 88 M values: fp32 residuals 2048 101 / 120, 8192 106 / 117 (RMS) and 115 / 121; half types with RMS
-  // norms 1024 117 / 124, 4096 121 / 127, but 5000 158 / 131, 8192 132 / 127, with LayerNorms 512 129 / 129, 768 136 / 144, but 1280 157 / 141, 4096 142 / 131,
-  // 8192 158 / 137, and rows that start at odd addresses, 333 359 / 283 and 304 / 230, 1999 279 / 245 and 241 / 206
-  const bool two = a.K > 8192 || (sizeof(R) == 2 && (a.K > 4096 || (a.K > 1024 && !a.rms) || (a.K > 256 && a.K % 8 != 0)));
+  // One piece to a thread / two, us at 88 M values (half of them onto fp32): fp32 residuals 1280 103 / 119, 2048 101 / 120, 8192 106 / 117; half types with RMS
+  // norms 333 197 / 152 (two rows share a wavefront), 1024 117 / 124, 1999 154 / 158, 4096 121 / 127, 5000 158 / 131, 8192 130 / 135, with LayerNorms 333 205 / 181, 512 129 /
+  // 129, 768 136 / 144, 1280 152 / 144, 2048 132 / 130, 4096 142 / 131, 5000 203 / 146, 8192 145 / 146
+  const bool two = a.K > 8192 || (sizeof(R) == 2 && (a.K > 4096 || (a.K > 1024 && !a.rms) || (a.K > 256 && a.K < 512)));
   return two ? go(N2{}) : go(N1{});
 }
 
@@ -274,6 +286,7 @@ extern "C" int samfast_norm_residual(const void* x, int64_t ldx, const void* res
   a.branch_scale = branch_scale;
   a.residual_scale = residual_scale;
   a.inv_K = 1.0f / (float)K;
+  a.in_place = total == x || total == residual;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == SAMFAST_F16) return residual_is_f32 ? launch_norm_residual<ElemF16, float>(a, s) : launch_norm_residual<ElemF16, us>(a, s);
   return residual_is_f32 ? launch_norm_residual<ElemBf16, float>(a, s) : launch_norm_residual<ElemBf16, us>(a, s);

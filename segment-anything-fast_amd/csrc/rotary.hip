@@ -23,6 +23,7 @@ struct RotaryArgs {
   const double* freq;   // axes * pairs, radians a position
   int64_t pos_b;
   float magnitude;
+  int in_place;
   int tokens, T, heads_q, heads, D, pairs, axes;
   int items;                  // a head's pieces; halves: the first `turns` of them are turned, `chunks` for an axis, the others copied
   int chunks, turns;
@@ -104,24 +105,30 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
     place(t, b, token);
     const RotarySide& s = a.side[h >= a.heads_q];
     if (h >= a.heads_q) h -= a.heads_q;
+    // (a piece that would end behind its like lies over the one before it, so that it is whole too: both write the same there)
     int d = item * kRotaryPiece;
     w.angle = t * angles;
     if (INTERLEAVED) {
+      if (a.D % 2 == 0 && a.D >= kRotaryPiece) d = min(d, a.D - kRotaryPiece);
       w.n = min(kRotaryPiece, a.D - d);
       w.angle += d / 2;
       w.turned = angles - d / 2;
     } else if (item < a.turns) {
       const int axis = a.axes == 1 ? 0 : item / a.chunks;
-      const int p = d - axis * a.chunks * kRotaryPiece;
+      int p = d - axis * a.chunks * kRotaryPiece;
+      if (a.pairs >= kRotaryPiece) p = min(p, a.pairs - kRotaryPiece);
       d = 2 * axis * a.pairs + p;
       w.angle += axis * a.pairs + p;
       w.turned = w.n = w.n2 = min(kRotaryPiece, a.pairs - p);
       w.second = a.pairs;
     } else {
+      const int last = a.D - 2 * angles >= kRotaryPiece ? a.D - kRotaryPiece : a.D;
       d = 2 * angles + (item - a.turns) * 2 * kRotaryPiece;
+      const int d2 = min(d + kRotaryPiece, last);
+      w.n2 = d + kRotaryPiece < a.D ? min(kRotaryPiece, a.D - d2) : 0;
+      d = min(d, last);
       w.n = min(kRotaryPiece, a.D - d);
-      w.second = kRotaryPiece;
-      w.n2 = max(min(kRotaryPiece, a.D - d - kRotaryPiece), 0);
+      w.second = d2 - d;
     }
     w.in = s.in + b * s.in_b + h * s.in_h + token * s.in_t + d;
     w.out = s.out + b * s.out_b + h * s.out_h + token * s.out_t + d;
@@ -149,6 +156,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
     sincospif(2.0f * (float)turns, &s, &c);
     table[table_at<PLANES>(i)] = f32x2{c * a.magnitude, s * a.magnitude};
   }
+  if (a.in_place) __builtin_amdgcn_s_waitcnt(0x0f70);  // (what two threads read is read before either of them writes)
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < EACH; ++u) {
@@ -217,6 +225,7 @@ extern "C" int samfast_rotary(const void* q, const void* k, void* q_out, void* k
   a.pos_b = pos_sb;
   a.tokens = (int)(B * T);
   a.magnitude = magnitude;
+  a.in_place = q_out == q || (k && k_out == k);
   a.T = (int)T;
   a.heads_q = heads_q;
   a.heads = heads_q + heads_k;

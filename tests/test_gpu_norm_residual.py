@@ -101,6 +101,21 @@ def test_in_place_strides_shapes_and_no_rows():
     assert none[0].shape == none[1].shape == (0, 200)
 
 
+@pytest.mark.parametrize("M,K", [(700, 5), (3000, 9), (2000, 333), (900, 1003), (500, 1999), (300, 5001), (100, 20001)])
+@pytest.mark.parametrize("norms", [0, 1, 2])
+def test_in_place_at_odd_widths(M, K, norms):
+    """Threads that share values of a row read them before one of them writes."""
+    from samfast_amd import ops
+    x, residual, gate, (post, pre) = _inputs(M, K, torch.bfloat16, torch.bfloat16, 1)
+    post, pre = post if norms > 0 else None, pre if norms > 1 else None
+    want = ops.norm_residual(x, residual, gate=gate, post=post, pre=pre, residual_scale=0.5)
+    for held in (residual, x):
+        mine = held.clone()
+        args = (mine, residual) if held is x else (x, mine)
+        total, normed = ops.norm_residual(*args, gate=gate, post=post, pre=pre, residual_scale=0.5, out=mine)
+        assert total is mine and torch.equal(mine, want[0]) and (pre is None or torch.equal(normed, want[1]))
+
+
 def test_a_row_that_is_not_finite_stays_alone():
     from samfast_amd import ops
     x, residual, gate, (post, pre) = _inputs(9, 1280, torch.bfloat16, torch.bfloat16, 1)

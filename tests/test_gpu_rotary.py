@@ -94,6 +94,22 @@ def test_in_place_and_layouts():
         assert ops.rotary(empty, None, p, freq)[0].shape == empty.shape
 
 
+@pytest.mark.parametrize("D,pairs,axes", [(6, 3, 1), (18, 9, 1), (66, 17, 1), (70, 11, 2), (84, 41, 1), (250, 102, 1), (45, 9, 2), (96, 13, 3), (30, 4, 1)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_in_place_at_odd_widths(D, pairs, axes, interleaved):
+    """Threads that share channels of a head read them before one of them writes."""
+    from samfast_amd import ops
+    q, k, _ = _qk(3, 7, 2, 211, D, torch.bfloat16)
+    q, k = q.contiguous(), k.contiguous()
+    positions = torch.arange(211 * axes, device="cuda").view(211, axes) * 3
+    freq = _frequencies(pairs, axes).view(axes, pairs)
+    want = ops.rotary(q, k, positions, freq, interleaved=interleaved)
+    for t, w in zip((q, k), want):
+        _check(w, t, positions, freq, interleaved, 1.0)
+    ops.rotary(q, k, positions, freq, interleaved=interleaved, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
 def test_position_zero_and_whole_turns_change_nothing():
     from samfast_amd import ops
     q, k, _ = _qk(1, 2, 1, 4, 64, torch.float16)
