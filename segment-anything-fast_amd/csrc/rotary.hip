@@ -35,6 +35,7 @@ constexpr int kRotaryThreads = 256;
 constexpr int kRotaryPiece = 8;       // values of 16 bytes
 constexpr int kRotaryTable = 1024;    // angles of a workgroup
 constexpr int kRotaryMaxDim = 1024;
+constexpr int kRotaryMaxAxes = 64;    // halves: a head has up to kRotaryMaxDim / 2 / kRotaryPiece + axes pieces, which a workgroup's threads have to hold
 // cosine and sine of the workgroup's angle i: a lane reads PLANES adjacent ones, which lie apart so that its neighbours' lie side by side
 template <int PLANES>
 SF_DEVICE int table_at(int i) { return i % PLANES * (kRotaryTable / PLANES + 1) + i / PLANES; }
@@ -67,7 +68,7 @@ SF_DEVICE float value(const u32x4& v, int e) { return e & 1 ? T::hi(v[e >> 1]) :
 template <class T, bool INTERLEAVED, int EACH>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   constexpr int PLANES = INTERLEAVED ? 4 : 8;
-  static_assert(kRotaryMaxDim / kRotaryPiece <= EACH * kRotaryThreads, "a workgroup has whole heads");
+  static_assert(kRotaryMaxDim / kRotaryPiece + kRotaryMaxAxes <= EACH * kRotaryThreads, "a workgroup has whole heads");
   __shared__ f32x2 table[kRotaryTable + PLANES];
   const int t0 = (int)blockIdx.x * a.block_tokens;
   const int nt = min(a.block_tokens, a.tokens - t0);
@@ -209,6 +210,7 @@ extern "C" int samfast_rotary(const void* q, const void* k, void* q_out, void* k
              "rotary: bad shape B=%lld T=%lld heads=%d, %d", (long long)B, (long long)T, heads_q, heads_k);
   SF_REQUIRE(axes >= 1 && pairs >= 1 && D >= 1 && D <= kRotaryMaxDim && (int64_t)2 * axes * pairs <= D,
              "rotary: %d axes of %d pairs do not fit into %d channels (at most %d)", axes, pairs, D, kRotaryMaxDim);
+  SF_REQUIRE(axes <= kRotaryMaxAxes, "rotary: %d axes (at most %d)", axes, kRotaryMaxAxes);
   SF_REQUIRE(strides, "rotary: null strides");
   if (B == 0 || T == 0 || heads_q + heads_k == 0) return SAMFAST_OK;
   SF_REQUIRE(B < (1ll << 31) / T, "rotary: too many tokens");

@@ -66,3 +66,8 @@ def _rotary(q=P, k=P, q_out=P, k_out=P, positions=P, pos_sb=0, frequencies=P, B=
     (dict(B=1 << 20, T=1 << 12), "too many tokens")])
 def test_rotary_refuses(change, text):
     _refused(_rotary(**change), text)
+
+
+def test_rotary_refuses_more_pieces_than_a_workgroup_holds():
+    _refused(_rotary(axes=65, pairs=1, D=256), "at most 64")
+    _refused(_rotary(axes=300, pairs=1, D=640), "at most 64")

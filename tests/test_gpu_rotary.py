@@ -149,3 +149,15 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="samfast"):
         ops.rotary(big, None, positions[:1], freq)
     assert math.isfinite(float(q.float().sum()))
+
+
+@pytest.mark.parametrize("D,pairs,axes", [(1024, 8, 64), (128, 1, 64), (1024, 1, 64), (1000, 7, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_axes(D, pairs, axes, interleaved):
+    from samfast_amd import ops
+    q, k, _ = _qk(2, 3, 1, 5, D, torch.bfloat16)
+    positions = torch.arange(5 * axes, device="cuda").view(5, axes)
+    freq = _frequencies(pairs, axes)
+    for o, t in zip(ops.rotary(q, k, positions, freq, interleaved=interleaved), (q, k)):
+        _check(o, t, positions, freq, interleaved, 1.0)
+        assert torch.equal(o[..., 2 * axes * pairs:], t[..., 2 * axes * pairs:])
