@@ -694,13 +694,40 @@ def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() == b.data_ptr() and a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride()
 
 
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two elements of t may share memory: no, where each axis steps over all that the smaller steps reach."""
+    reach = 1
+    for step, n in sorted((abs(s), n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if step < reach:
+            return True
+        reach += step * (n - 1)
+    return False
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether no byte belongs to both: they lie one behind the other, or take turns in windows of one step that both have (the queries' and the keys'
+    heads of each token in one buffer)."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if max(a0, b0) >= min(a1, b1):
+        return True
+    size = a.element_size()
+    if size != b.element_size() or (b0 - a0) % size != 0:
+        return False
+    axes = [[(s, n) for n, s in zip(t.shape, t.stride()) if n > 1] for t in (a, b)]
+    for step in {s for one in axes for s, _ in one if s > 0}:
+        if any(s > step and s % step != 0 for one in axes for s, _ in one):
+            continue
+        width_a, width_b = (1 + sum(s * (n - 1) for s, n in one if s < step) for one in axes)
+        ahead = (b0 - a0) // size % step
+        if width_a <= ahead and ahead + width_b <= step:
+            return True
+    return False
+
+
 def _check_out(name: str, out: torch.Tensor, own: Sequence[torch.Tensor], others: Sequence[Optional[torch.Tensor]]) -> None:
-    """`out` is one of `own`, or lies apart from all of `own` and `others`, and no two of its elements share memory."""
-    if any(_same_view(out, t) for t in own):
-        return
-    a, b = _span(out)
-    clash = any(t is not None and max(a, _span(t)[0]) < min(b, _span(t)[1]) for t in (*own, *others))
-    if clash or torch._debug_has_internal_overlap(out) == 1:
+    """Each of `own` is `out` or lies apart from it, `others` lie apart from it, and no two of its elements share memory."""
+    clash = any(not _same_view(out, t) and not _apart(out, t) for t in own) or any(t is not None and not _apart(out, t) for t in others)
+    if clash or _overlaps_itself(out):
         raise RuntimeError(f"samfast: {name}'s out overlaps itself or an input in another way than being one")
 
 
@@ -844,11 +871,13 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         outs = [torch.empty((B, T, t.shape[1], D), dtype=t.dtype, device=t.device).permute(0, 2, 1, 3) for t in tensors]
     else:
         outs = list(out[:len(tensors)])
+        if len(outs) != len(tensors):
+            raise RuntimeError("samfast: out must hold a tensor for q and one for k")
         for t, o in zip(tensors, outs):
             if o is None or o.shape != t.shape or o.dtype != t.dtype:
                 raise RuntimeError("samfast: out must hold tensors of q's and k's shapes and dtype")
         for i, (t, o) in enumerate(zip(tensors, outs)):
-            _check_out("rotary", o, (t,), (*tensors, positions, frequencies, *outs[:i], *outs[i + 1:]))
+            _check_out("rotary", o, (t,), (*tensors[:i], *tensors[i + 1:], positions, frequencies, *outs[:i], *outs[i + 1:]))
     strides = []
     for t, o in zip(tensors, outs):
         strides += [*_bnhd_strides(t), *_bnhd_strides(o)]
