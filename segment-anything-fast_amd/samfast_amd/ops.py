@@ -757,9 +757,10 @@ def linear_i4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
         raise RuntimeError(f"samfast: linear_i4 bias must be fp32 of length {N}")
     rows = x.reshape(-1, K)
-    if rows.stride(1) != 1 or rows.stride(0) % 8 != 0 or rows.stride(0) < K or rows.data_ptr() % 16 != 0:
-        rows = rows.clone(memory_format=torch.contiguous_format)
     M = rows.shape[0]
+    step = rows.stride(0) if M > 1 else K
+    if rows.stride(1) != 1 or step % 8 != 0 or not K <= step < 1 << 22 or rows.data_ptr() % 16 != 0:  # (rows further apart: offsets in a tile are 32 bits)
+        rows, step = rows.clone(memory_format=torch.contiguous_format), K
     lib = _lib.load()
     need = lib.samfast_linear_i4_workspace(M, N, K)
     if need < 0:
@@ -769,7 +770,7 @@ def linear_i4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     code = _timed(
         "linear_i4", 2.0 * M * N * K, "flop",
         lambda: lib.samfast_linear_i4(
-            rows.data_ptr(), rows.stride(0), codes.data_ptr(), scales.data_ptr(), zeros.data_ptr() if zeros is not None else None,
+            rows.data_ptr(), step, codes.data_ptr(), scales.data_ptr(), zeros.data_ptr() if zeros is not None else None,
             bias.data_ptr() if bias is not None else None, y.data_ptr(), N, work.data_ptr() if work is not None else None,
             M, N, K, group_size, dtype, _stream()))
     _lib.check(code, "linear_i4")

@@ -121,3 +121,16 @@ def test_refusals():
             ops.linear_i4(*args, group_size=group)
     with torch.no_grad():
         ops.linear_i4(x.clone().requires_grad_(), codes, scales, z, b, group_size=64)
+
+
+@pytest.mark.parametrize("M", [1, 3, 40])
+def test_rows_far_apart(M):
+    """The last tokens of long prompts: rows that lie megabytes apart."""
+    from samfast_amd import ops
+    x, codes, scales, z, b = _operands(M, 512, 96, 64, True, torch.bfloat16)
+    prompts = torch.zeros((M, 8200, 512), dtype=x.dtype, device="cuda")
+    prompts[:, -1] = x
+    want = ops.linear_i4(x, codes, scales, z, b, group_size=64)
+    assert torch.equal(ops.linear_i4(prompts[:, -1], codes, scales, z, b, group_size=64), want)
+    with ops.record_launches():
+        assert torch.equal(ops.linear_i4(prompts[:, -1:], codes, scales, z, b, group_size=64), want.view(M, 1, 96))
