@@ -341,7 +341,9 @@ static int launch_i4_tiled(I4Args a, const I4Plan& plan, hipStream_t stream) {
     using P = I4Tile<decltype(mt)::value, decltype(nt)::value, decltype(cols)::value, decltype(sides)::value>;
     a.tiles_m = (a.M + P::BM - 1) / P::BM;
     a.tiles_n = (a.N + P::BN - 1) / P::BN;
-    const dim3 grid((unsigned int)(((int64_t)a.tiles_m * a.tiles_n + 7) / 8 * 8), (unsigned int)plan.splits);
+    const int64_t tiles = ((int64_t)a.tiles_m * a.tiles_n + 7) / 8 * 8;
+    SF_REQUIRE(launchable(tiles, P::THREADS), "linear_i4: %lld tiles are too many for a launch", (long long)tiles);
+    const dim3 grid((unsigned int)tiles, (unsigned int)plan.splits);
     hipLaunchKernelGGL((linear_i4_kernel<T, decltype(mt)::value, decltype(nt)::value, decltype(cols)::value, decltype(sides)::value>), grid,
                        dim3(P::THREADS), 0, stream, a);
     if (const int rc = check_launch("linear_i4_kernel")) return rc;

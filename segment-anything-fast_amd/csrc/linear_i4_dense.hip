@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void i4_weights_kernel(I4Args a, unsigned shor
 // The time: a launch, the weights read and written, and pp_choose's cost, a unit of which takes 0.085 us where the GPU is nearly idle and 0.115 where it is
 // busy throughout (power).  2048 x 4096 -> 4096 72 us, 4096 x 1280 -> 5120 50, 65536 x 1280 -> 3840 479, 1024 x 8192 -> 8192 153.
 int i4_dense_tile(int64_t M, int N, int K, double* time) {
-  if (K % 64 != 0 || K < 320 || N % 8 != 0 || M < 256) return 0;
+  if (K % 64 != 0 || K < 320 || N % 8 != 0 || M < 256 || !launchable((int64_t)N * (K / 8) / 256 + 1, 256)) return 0;
   const PPChoice c = pp_choose(M, N, K / 64, false, 8.1);
   if (c.tn == 0) return 0;
   const double fragments = c.tn == 10 ? 12.5 : c.tn == 8 ? 10.0 : 8.1;

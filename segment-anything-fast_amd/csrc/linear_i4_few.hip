@@ -290,6 +290,7 @@ template <class T, int MT, int NT>
 static int go_few(const I4Args& a, hipStream_t stream) {
   const int units = (a.K + 255) / 256, waves = units < kI4FewWaves ? units : kI4FewWaves;
   const dim3 grid((unsigned int)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned int)((a.M + 16 * MT - 1) / (16 * MT)));
+  SF_REQUIRE(launchable(grid.x, 64 * waves), "linear_i4: %d outputs are too many for a launch", a.N);
   auto go = [&](auto steps) {
     hipLaunchKernelGGL((linear_i4_few_kernel<T, MT, NT, decltype(steps)::value>), grid, dim3(64 * waves), 0, stream, a);
     return check_launch("linear_i4_few_kernel");

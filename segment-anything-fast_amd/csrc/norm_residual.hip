@@ -231,6 +231,7 @@ static int launch_norm_residual(NormResidualArgs a, hipStream_t stream) {
     a.halves = (a.K + 256 * NCH - 1) / (256 * NCH);
     a.rows = a.halves % 2 == 1 && a.halves <= 15 ? 2 : 1;
     const dim3 grid((unsigned int)((a.M + a.rows - 1) / a.rows)), block((a.rows * a.halves + 1) / 2 * 64);
+    SF_REQUIRE(launchable(grid.x, (int)block.x), "norm_residual: %lld rows are too many for a launch", (long long)a.M);
     if (a.K % 8 == 0) hipLaunchKernelGGL((norm_residual_kernel<T, R, NCH, true>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((norm_residual_kernel<T, R, NCH, false>), grid, block, 0, stream, a);
     return check_launch("norm_residual_kernel");
@@ -264,6 +265,8 @@ extern "C" int samfast_norm_residual(const void* x, int64_t ldx, const void* res
   SF_REQUIRE(post_eps >= 0.f && pre_eps >= 0.f, "norm_residual: eps must not be negative");
   SF_REQUIRE(M == 0 || (x && residual && total), "norm_residual: null pointer");
   SF_REQUIRE(ldx >= K && ld_res >= K, "norm_residual: row strides must hold a row");
+  SF_REQUIRE(M <= 1 || ((total != residual || ld_res == K) && (total != x || (ldx == K && !residual_is_f32))),
+             "norm_residual: total lies where its rows are read in another layout");
   if (M == 0) return SAMFAST_OK;
   NormResidualArgs a = {};
   a.x = (const us*)x;

@@ -252,6 +252,11 @@ extern "C" int samfast_rotary(const void* q, const void* k, void* q_out, void* k
   SF_REQUIRE(parts < 65536, "rotary: too many heads");
   a.div_items = a.items > 1 ? divider(a.items) : 0;
   a.div_heads = a.block_heads > 1 ? divider(a.block_heads) : 0;
+  SF_REQUIRE(launchable((a.tokens + a.block_tokens - 1) / a.block_tokens, kRotaryThreads), "rotary: too many tokens");
+  for (int i = 0; i < 2; ++i) {
+    const RotarySide& t = a.side[i];
+    SF_REQUIRE(!t.out || t.out != t.in || (t.out_b == t.in_b && t.out_h == t.in_h && t.out_t == t.in_t), "rotary: in place, but in another layout");
+  }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return dtype == SAMFAST_F16 ? launch_rotary<ElemF16>(a, interleaved != 0, s) : launch_rotary<ElemBf16>(a, interleaved != 0, s);
 }

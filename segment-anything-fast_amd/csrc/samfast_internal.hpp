@@ -22,6 +22,9 @@ void set_error(const char* fmt, ...);
 
 int check_launch(const char* what);
 
+// a grid's x axis has fewer than 2^32 threads
+static inline bool launchable(int64_t blocks, int threads) { return blocks < (1ll << 32) / threads; }
+
 // Tuning knobs: each is an environment variable read ONCE (at the first query of any knob), after
 // which samfast_bench_set_knob (include/samfast_bench.h) is the only way to change it.
 enum Knob {

@@ -15,7 +15,7 @@ def _refused(code, text):
     assert code < 0 and text in lib.samfast_last_error().decode(), (code, lib.samfast_last_error())
 
 
-P = 0x1000  # an aligned address that is never read
+P, Q = 0x1000, 0x2000  # aligned addresses that are never read
 
 
 def _linear(x=P, ldx=64, codes=P, scales=P, zeros=None, bias=None, y=P, ldy=40, work=P, M=2, N=40, K=64, group=32, dtype=0):
@@ -40,9 +40,9 @@ def test_no_rows_are_accepted_without_memory():
 
 
 def _norm(x=P, ldx=64, residual=P, ld_res=64, gate=None, gate_rows=1, post=None, post_beta=None, post_eps=0.0, pre=P, pre_beta=None, pre_eps=0.0,
-          total=P, normed=P, M=6, K=64, dtype=0):
+          total=P, normed=P, M=6, K=64, dtype=0, f32=0):
     return _lib().samfast_norm_residual(x, ldx, residual, ld_res, gate, gate_rows, post, post_beta, post_eps, pre, pre_beta, pre_eps, 0, 1.0, 1.0,
-                                        total, normed, M, K, dtype, 0, None)
+                                        total, normed, M, K, dtype, f32, None)
 
 
 @pytest.mark.parametrize("change,text", [
@@ -71,3 +71,22 @@ def test_rotary_refuses(change, text):
 def test_rotary_refuses_more_pieces_than_a_workgroup_holds():
     _refused(_rotary(axes=65, pairs=1, D=256), "at most 64")
     _refused(_rotary(axes=300, pairs=1, D=640), "at most 64")
+
+
+@pytest.mark.parametrize("change", [dict(M=1 << 30, N=1, K=8, ldx=8, ldy=1), dict(M=1, N=1 << 29, K=4096, ldx=4096, ldy=1 << 29)])
+def test_linear_i4_refuses_what_no_launch_holds(change):
+    _refused(_linear(**change), "too many for a launch")
+
+
+def test_norm_residual_and_rotary_refuse_what_no_launch_holds():
+    _refused(_norm(M=(1 << 31) - 1), "too many for a launch")
+    _refused(_rotary(B=1, T=(1 << 31) - 2, D=1024, pairs=512, axes=1), "too many tokens")
+
+
+@pytest.mark.parametrize("change", [dict(ld_res=72), dict(total=Q, x=Q, ldx=72), dict(total=Q, x=Q, f32=1)])
+def test_norm_residual_refuses_a_total_over_rows_of_another_layout(change):
+    _refused(_norm(**change), "another layout")
+
+
+def test_rotary_refuses_in_place_in_another_layout():
+    _refused(_rotary(), "another layout")
