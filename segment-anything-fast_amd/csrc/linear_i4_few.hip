@@ -2,8 +2,11 @@
 //
 // A workgroup has 16 NT columns, its wavefronts take turns over K in segments of 128.  A lane loads 16 bytes of codes, 32 adjacent k of one
 // column; four lanes that hold one column exchange words (v_permlane32_swap, v_permlane16_swap) until each 16 x 16 x 32 matrix instruction
-// multiplies 32 adjacent k, which belong to one group.  code - zero is exact in either type; a group's sum is scaled in fp32, so no weight is
-// rounded.  The wavefronts' sums meet in LDS.
+// multiplies 32 adjacent k, which belong to one group.  The codes are exact in either type; a group's sum is scaled in fp32, and its zero times the
+// group's sum of x taken off in fp32, so no weight is rounded.  The wavefronts' sums meet in LDS.
+//
+// us (a copy's time for the weights): 1 x 4096 -> 4096 5.1 (1.7), 1 x 8192 -> 8192 9.2 (6.7), with zeros and groups of 32 11.9 (7.7); 24 rows of the last 16.4: 100 MB of x out of the
+// L2s, a workgroup's own rows for each, and about 500 vector instructions for 256 k of two fragments of columns.
 #include "linear_i4_shared.hpp"
 
 #include <type_traits>
@@ -35,7 +38,7 @@ SF_DEVICE u32x4 i4_numbers(unsigned int w) {
 // A wavefront takes 256 k at a time, and the next ones are under way while it multiplies.  The rows of x go straight into LDS of its own, whole lines
 // to a load, and from there into registers: fragments straight from memory are half lines, and 24 x 8192 x 8192 took 22 us instead of 14.  (Codes
 // as fragments or as lines were level.)  Scales and zeros come four columns of a group to a lane, and are handed round by way of LDS: as each lane's own,
-// a load for each group, groups of 32 took 19.6 us instead of 18.0 there.  The loop has no branches, and addresses are uniform bases with 32-bit offsets that are made once: with a K that
+// a load for each group, groups of 32 took 19.6 us instead of 18.0 there (16.4 now).  The loop has no branches, and addresses are uniform bases with 32-bit offsets that are made once: with a K that
 // may end anywhere inside it, the loads of all paths were waited for at each step, and 1 x 8192 x 8192 took 16 us instead of 11.  What is left of K goes
 // through a loop of its own.
 constexpr int kI4FewWaves = 8;
@@ -120,22 +123,37 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
     load_scales(w, 8 * p);
   };
   f32x4 acc[MT][NT];
-  // The products of 128 k, the h-th of those whose scales, and these times the zeros, were handed round.  SIMPLE: code - zero is made before it is multiplied, with the lane's own column's zero; else the codes are, and
-  // the zero times the group's sum of x, which all columns share, is taken off.
+  // The zeros' part of 256 k: the groups' sums of x, which all columns share, times -scale * zero, four groups to an instruction in fp32.  Row n of the
+  // sums' first operand has ones for the group that lanes of quarter n / 4 take along, and all groups add to one register.  (As vector instructions on each
+  // group's sum 24 x 8192 -> 8192 17.4 us for 16.4, in groups of 64 14.9 for 14.0; before the products 16.6.)
+  constexpr unsigned int ones = T::kOne | T::kOne << 16;
+  unsigned int picks[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) picks[q] = lr >> 2 == q ? ones : 0u;
+  auto take_zeros_off = [&](const u32x4 (&x)[2][MT][4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 2 * GROUPS; c += 4) {
+      f32x4 sum[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) sum[i] = f32x4{};
+#pragma unroll
+      for (int q = 0; q < 4 && c + q < 2 * GROUPS; ++q)
+#pragma unroll
+        for (int s = (c + q) * STEPS; s < (c + q + 1) * STEPS; ++s)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) sum[i] = T::mfma16(u32x4{picks[q], picks[q], picks[q], picks[q]}, x[s >> 2][i][s & 3], sum[i]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const float sz = reinterpret_cast<const float*>(mine + XBYTES + 1024)[(c + lq) * 4 * Q + 16 * j + lr];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(sz, sum[i][0], acc[i][j], 0, 0, 0);
+      }
+    }
+  };
+  // The products of 128 k, the h-th of those whose scales were handed round.  SIMPLE: code - zero is made before it is multiplied, with the lane's own
+  // column's zero; else the codes are.
   auto multiply = [&](const u32x4 (&cw)[NT], const u32x4 (&x)[MT][4], int h, int seg, auto simple, unsigned int zeros = 0) __attribute__((always_inline)) {
     constexpr bool SIMPLE = decltype(simple)::value;
-    f32x4 sum[GROUPS][MT];
-    if constexpr (!SIMPLE) {
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          sum[g][i] = f32x4{};
-          constexpr unsigned int one = T::kOne | T::kOne << 16;
-#pragma unroll
-          for (int t = g * STEPS; t < (g + 1) * STEPS; ++t) sum[g][i] = T::mfma16(u32x4{one, one, one, one}, x[i][t], sum[g][i]);
-        }
-    }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       u32x4 c = cw[j];
@@ -168,13 +186,6 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(part[i][e], s[e], acc[i][j][e]);
-        if constexpr (!SIMPLE) {
-          const f32x4 sz = reinterpret_cast<const f32x4*>(mine + XBYTES)[64 + from + lq];
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[g][i][e], sz[e], acc[i][j][e]);
-        }
       }
     }
   };
@@ -239,6 +250,7 @@ __global__ __launch_bounds__(64 * kI4FewWaves) void linear_i4_few_kernel(I4Args 
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) multiply(now.codes[h], x[h], h, 2 * unit(n) + h, std::false_type{});
+      take_zeros_off(x);
     }
   }
   // An infinity in a row or a scale, or sums that overflow before the zero is taken off, end as a NaN or an infinity here; the simple
