@@ -1,10 +1,12 @@
 /*
  * samfast - C ABI of the MI355X (gfx950) SAM image-encoder hot path.
  *
- * Two groups of entry points:
+ * Three groups of entry points:
  *   attention with decomposed relative-position bias (global 64-wide grids and
- *   small windows), and dynamic symmetric int8 linears (row quantiser, int8
- *   GEMM with int32 accumulators, fused scale+bias epilogue).
+ *   small windows), dynamic symmetric int8 linears (row quantiser, int8
+ *   GEMM with int32 accumulators, fused scale+bias epilogue), and what stands
+ *   around attention in other blocks: linears with 4-bit weights, norms over a
+ *   gated residual, rotary positions.
  *
  * Conventions
  *   - every pointer is a DEVICE pointer unless named host_*; the caller owns
@@ -243,11 +245,11 @@ int samfast_linear_half(
  *   y[m, n] = sum_g scales[g, n] * sum_{k in g} x[m, k] * (code[n, k] - zeros[g, n]) + bias[n],   group g = inputs g * group and on,
  * summed in fp32 and rounded to `dtype` once.  codes (N, K/2) contiguous, two to a byte, the even input in the lower half; scales
  * (ceil(K / group), N) of type `dtype`, contiguous; zeros (ceil(K / group), N) uint8 or NULL, which stands for 8 throughout; bias fp32 (N)
- * or NULL.  K % 8 == 0, group % 32 == 0 (the last group may be shorter); any N.  x has row stride ldx, a multiple of 8, and is 16-byte
- * aligned, codes and bias are 4-byte aligned; y has row stride ldy, any.  `workspace`: samfast_linear_i4_workspace(M, N, K) bytes of device
- * memory, 16-byte aligned, contents irrelevant before and after; NULL where that is 0.
- * Over more than SAMFAST_I4_FEW_ROWS rows the weights (code - zero) * scale are rounded to `dtype` before they are
- * multiplied: in fp16 they have to stay below 65504 there.
+ * or NULL.  K % 8 == 0, K <= 2^20, group % 32 == 0 (the last group may be shorter); any N.  x has row stride ldx, a multiple of 8 below 2^22, and is
+ * 16-byte aligned, codes and bias are 4-byte aligned; y has row stride ldy, any.  `workspace`: samfast_linear_i4_workspace(M, N, K) bytes of device
+ * memory, 16-byte aligned, contents irrelevant before and after, for one call at a time; NULL where that is 0.
+ * Over more than SAMFAST_I4_FEW_ROWS rows, and for fewer than 16 outputs, the weights (code - zero) * scale are rounded to `dtype` before they are
+ * multiplied, and have to be finite in it: below 65504 in fp16.
  */
 #define SAMFAST_I4_FEW_ROWS 32
 int64_t samfast_linear_i4_workspace(int64_t M, int N, int K);
@@ -262,7 +264,7 @@ int samfast_linear_i4(
  * out where its gamma is NULL (normed is then NULL too); a NULL beta is none.  x, gate, norm weights and normed are of type `dtype`, residual and
  * total of it too or, with residual_is_f32, fp32.  gate: gate_rows rows of K, each for M / gate_rows rows, or NULL.  x and residual have row strides
  * ldx and ld_res, the others are contiguous; any alignment.  fp32 throughout, pre of the total before it is
- * rounded.  total may be the residual's memory (then ld_res == K).
+ * rounded.  total may be the residual's memory (then ld_res == K), or x's (then ldx == K and both of one type), and shares none otherwise.
  */
 int samfast_norm_residual(
     const void* x, int64_t ldx, const void* residual, int64_t ld_res, const void* gate, int64_t gate_rows,
@@ -276,7 +278,8 @@ int samfast_norm_residual(
  * the others are copied.  An axis has 2 * pairs adjacent channels; its pairs are neighbours (`interleaved`) or a channel of the lower half and its
  * like of the upper.  q and k are addressed as ptr + b*s_b + h*s_h + t*s_t + d; `strides` (host memory, read before the call returns): s_b, s_h, s_t of q,
  * of q_out, of k, of k_out, in elements.  positions int64, axes a token, tokens contiguous, pos_sb between images (0: all the
- * same); frequencies fp64 (axes, pairs).  The angle is made in fp64.  Any alignment.  q_out and k_out may be q and k.  With heads_k = 0 q alone.  D <= 1024.
+ * same); frequencies fp64 (axes, pairs).  The angle is made in fp64.  Any alignment.  q_out and k_out may be q and k, with their strides, and share no
+ * memory otherwise.  With heads_k = 0 q alone.  D <= 1024, axes <= 64.
  */
 int samfast_rotary(
     const void* q, const void* k, void* q_out, void* k_out, const int64_t* positions, int64_t pos_sb, const double* frequencies,

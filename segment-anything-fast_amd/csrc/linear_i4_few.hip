@@ -1,6 +1,6 @@
 // Linears with 4-bit weights over few rows, the steps of token generation: the weights are read once and bound it, the rows come out of the L2s.
 //
-// A workgroup has 16 NT columns, its wavefronts take turns over K in segments of 128.  A lane loads 16 bytes of codes, 32 adjacent k of one
+// A workgroup has 16 NT columns, its wavefronts take turns over K, 256 at a time.  A lane loads 16 bytes of codes, 32 adjacent k of one
 // column; four lanes that hold one column exchange words (v_permlane32_swap, v_permlane16_swap) until each 16 x 16 x 32 matrix instruction
 // multiplies 32 adjacent k, which belong to one group.  The codes are exact in either type; a group's sum is scaled in fp32, and its zero times the
 // group's sum of x taken off in fp32, so no weight is rounded.  The wavefronts' sums meet in LDS.

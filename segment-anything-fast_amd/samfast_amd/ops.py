@@ -735,7 +735,8 @@ def linear_i4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
               bias: Optional[torch.Tensor] = None, *, group_size: int) -> torch.Tensor:
     """Linear with 4-bit weights on half-type rows x (..., K): y = x w^T + bias with w[n, k] = (code[n, k] - zeros[g, n]) * scales[g, n],
     g = k // group_size.  codes: uint8 (N, K/2), the even k in the lower half of a byte; scales (groups, N) of x's dtype; zeros uint8 (groups, N),
-    or None for 8; bias fp32 (N).  K a multiple of 8, group_size of 32; the last group may be shorter.  Returns (..., N)."""
+    or None for 8; bias fp32 (N).  K a multiple of 8 up to 2^20, group_size of 32; the last group may be shorter.  fp32 sums; up to 32 rows of x (of 16
+    outputs or more) the weights are exact, over more they are rounded to x's dtype.  Returns (..., N)."""
     if _launch_log is None:
         y = (_lib._host or _lib.host()).linear_i4(x, codes, scales, zeros, bias, group_size)
         if y is not None:
@@ -845,9 +846,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
            scale: float = 1.0, out: Optional[Tuple[torch.Tensor, Optional[torch.Tensor]]] = None):
     """Rotary positions in queries and keys: q (B, nH, T, hd) and k (B, nKV, T, hd), any batch / head / token strides (head_dim contiguous), half
     types.  positions int64, (B, T) or (T,); frequencies fp64 (pairs,), radians a position.  For a grid positions (..., T, axes) and
-    frequencies (axes, pairs).  Axis after axis, 2 * pairs channels of the head are turned: pairs of neighbours (`interleaved`), or of a channel
+    frequencies (axes, pairs), axes <= 64.  Axis after axis, 2 * pairs channels of the head are turned: pairs of neighbours (`interleaved`), or of a channel
     and its like half of the axis's channels on; channels behind the last axis's are copied.  `scale` multiplies what is turned.  Angles are made in 64
-    bits.  Returns (q', k') in q's and k's shapes, laid out token-major (k' is None where k is), or in `out`, whose tensors are q and k themselves or memory of their own."""
+    bits.  Returns (q', k') in q's and k's shapes, laid out token-major (k' is None where k is), or in `out`, whose tensors are q and k themselves or memory of their own.  Head dims up to 1024."""
     if out is None and _launch_log is None:
         both = (_lib._host or _lib.host()).rotary(q, k, positions, frequencies, interleaved, scale)
         if both is not None:
