@@ -74,3 +74,15 @@ def test_frequencies_and_grid():
         with pytest.raises(ValueError):
             rotary_frequencies(**bad)
     assert grid_positions(2, 3).tolist() == [[0, 0], [0, 1], [0, 2], [1, 0], [1, 1], [1, 2]]
+
+
+def test_a_model_is_swapped_whole_or_not_at_all():
+    from samfast_amd import Int4Linear, apply_int4_weights
+    model = torch.nn.Sequential(torch.nn.Linear(64, 12), torch.nn.ReLU(), torch.nn.Linear(12, 8))
+    with pytest.raises(ValueError, match="2: "):
+        apply_int4_weights(model)
+    with pytest.raises(ValueError):
+        apply_int4_weights(model, lambda mod, fqn: fqn == "0", group_size=48)
+    assert [type(m) for m in model] == [torch.nn.Linear, torch.nn.ReLU, torch.nn.Linear]
+    apply_int4_weights(model, lambda mod, fqn: fqn == "0")
+    assert isinstance(model[0], Int4Linear) and isinstance(model[2], torch.nn.Linear)
