@@ -247,7 +247,7 @@ int samfast_linear_half(
  * (ceil(K / group), N) of type `dtype`, contiguous; zeros (ceil(K / group), N) uint8 or NULL, which stands for 8 throughout; bias fp32 (N)
  * or NULL.  K % 8 == 0, K <= 2^20, group % 32 == 0 (the last group may be shorter); any N.  x has row stride ldx, a multiple of 8 below 2^22, and is
  * 16-byte aligned, codes and bias are 4-byte aligned; y has row stride ldy, any.  `workspace`: samfast_linear_i4_workspace(M, N, K) bytes of device
- * memory, 16-byte aligned, contents irrelevant before and after, for one call at a time; NULL where that is 0.
+ * memory (weights, sums or rows of x), 16-byte aligned, contents irrelevant before and after, for one call at a time; NULL where that is 0.
  * Over more than SAMFAST_I4_FEW_ROWS rows, and for fewer than 16 outputs, the weights (code - zero) * scale are rounded to `dtype` before they are
  * multiplied, and have to be finite in it: below 65504 in fp16.
  */

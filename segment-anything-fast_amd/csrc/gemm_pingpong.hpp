@@ -342,6 +342,8 @@ __global__ __launch_bounds__(512, 2) void gemm_pingpong_kernel(PPArgs a) {
   // wavefronts share a SIMD's vector unit.  Where the conversion is an add and half a pack per value, they finish one behind the other,
   // each under a turn of the other's products.
   constexpr bool TOGETHER = E::SCALED || EPI != PP_PLAIN;
+  // with an fp32 bias any number of columns: a quad or pair that begins in the tile before is stored by both, with the same bits
+  constexpr int OVER = E::BIAS32 ? 1 : 0;
   auto finish = [&](auto whole) __attribute__((always_inline)) {
     constexpr bool FULL = decltype(whole)::value;
     const int l = lane_again(), lr = l & 15, lq = l >> 4;
@@ -410,7 +412,7 @@ __global__ __launch_bounds__(512, 2) void gemm_pingpong_kernel(PPArgs a) {
           const u32x2 v = RES ? res[RES ? i : 0][r][g] : u32x2{0u, 0u};
           const u32x2 o = {two(r, g, 0, v[0]), two(r, g, 2, v[1])};
           const gquad_t dst = (gquad_t)to.at(g);
-          if (FULL || (row >= skip_m && col0 + 64 * g + 4 * lr >= skip_n)) {
+          if (FULL || (row >= skip_m && col0 + 64 * g + 4 * lr + OVER * 3 >= skip_n)) {
             if (NT) __builtin_nontemporal_store(o, dst);
             else *dst = o;
           }
@@ -418,7 +420,7 @@ __global__ __launch_bounds__(512, 2) void gemm_pingpong_kernel(PPArgs a) {
         if constexpr (P::PAIR) {
           const unsigned int o = two(r, P::NQ, 0, RES ? res_pair[RES ? i : 0][r] : 0u);
           const gpair_t dst = (gpair_t)to.at(P::NQ);
-          if (FULL || (row >= skip_m && col0 + 64 * P::NQ + 2 * lr >= skip_n)) {
+          if (FULL || (row >= skip_m && col0 + 64 * P::NQ + 2 * lr + OVER >= skip_n)) {
             if (NT) __builtin_nontemporal_store(o, dst);
             else *dst = o;
           }

@@ -300,10 +300,10 @@ __global__ __launch_bounds__(256) void i4_sum_kernel(I4Args a, int splits) {
 // a fifth of the times measured.
 //   tiles: 4 + a k tile's time x k tiles x tiles to a CU, alone on it / not; + 3 and the sums' bytes at 6 TB/s where K is split.  Measured, 32 x 64 / 64 x 64 /
 //     128 x 128 tiles: 128 x 1280 -> 3840 7.0 / 8.5 / 12, 333 x 1000 -> 1003 7.5 / 8.8 / 12, 256 x 4096 -> 4096 23.5 / 20.9 / 23 (K split), 512 x 4096 -> 4096
-//     - / 31.2 / 33, 1024 x 1280 -> 3840 - / 22.3 / 18.0, 8000 x 4096 -> 3001 - / 262 / 197; K whole / in four: 64 x 4096 -> 4096 20 / 11.9, 64 x 8192 -> 8192 35 / 20.9,
+//     - / 31.2 / 33, 1024 x 1280 -> 3840 - / 22.3 / 18.0, 8000 x 4096 -> 3001 - / 262 / 242; K whole / in four: 64 x 4096 -> 4096 20 / 11.9, 64 x 8192 -> 8192 35 / 20.9,
 //     256 x 4096 -> 4096 20.9 / 24.
-//   dense (linear_i4_dense.hip): by its own estimate.  tiles / dense: 4096 x 1280 -> 5120 58 / 50, 16384 x 1280 -> 5120 204 / 160, but 4096 x 1280 -> 1280 25 / 33,
-//     1024 x 8192 -> 8192 135 / 153.
+//   dense (linear_i4_dense.hip): by its own estimate.  tiles / dense: 4096 x 1280 -> 5120 73 / 50, 5405 x 3832 -> 4828 267 / 180, 8000 x 4096 -> 3001 242 / 157,
+//     4096 x 1280 -> 5121 84 / 57, 10000 x 328 -> 4001 63 / 49, 1024 x 8192 -> 8192 162 / 146, but 1024 x 4096 -> 4096 50 / 65, 512 x 8192 -> 8192 92 / 128, 4096 x 1280 -> 1280 26 / 28.
 // Up to SAMFAST_I4_FEW_ROWS rows linear_i4_few.hip: 24 x 4096 -> 4096 7.7, tiles 15.
 struct I4Plan {
   int dense;   // columns / 32 of the dense product's tile, or 0
@@ -331,6 +331,8 @@ static I4Plan i4_plan(int64_t M, int N, int K) {
     }
   double dense = 0.0;
   const int columns = i4_dense_tile(M, N, K, &dense);
+  // (against the dense product the estimate of the largest tiles is too short: their ends, and the power limit from a round of them on; 16384 x 1000 -> 1003 52, 36 above)
+  if (p.tile == 2) least = 1.18 * (least - 4.0) + 4.0 + 2.0 * fmax((double)((M + 127) / 128) * ((N + 127) / 128) / 256.0 - 1.0, 0.0);
   if (columns && dense < least) p = I4Plan{columns, 0, 1};
   return p;
 }
@@ -366,7 +368,7 @@ extern "C" int64_t samfast_linear_i4_workspace(int64_t M, int N, int K) {
   using namespace samfast;
   SF_REQUIRE(M >= 0 && N > 0 && K > 0, "linear_i4_workspace: bad shape M=%lld N=%d K=%d", (long long)M, N, K);
   const I4Plan plan = i4_plan(M, N, K);
-  return plan.dense ? (int64_t)N * K * 2 : plan.splits > 1 ? (int64_t)plan.splits * M * N * 4 : 0;
+  return plan.dense ? i4_dense_workspace(M, N, K) : plan.splits > 1 ? (int64_t)plan.splits * M * N * 4 : 0;
 }
 
 extern "C" int samfast_linear_i4(const void* x, int64_t ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros, const float* bias,
@@ -400,7 +402,7 @@ extern "C" int samfast_linear_i4(const void* x, int64_t ldx, const uint8_t* code
   a.group = group;
   a.div_group = i4_divider(group < K ? group : (K + 31) / 32 * 32);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (plan.dense && ldy % 8 == 0 && ldy < (1 << 22) && aligned16(y)) return launch_i4_dense(a, dtype == SAMFAST_F16, plan.dense, workspace, s);
+  if (plan.dense && ldy < (1 << 22)) return launch_i4_dense(a, dtype == SAMFAST_F16, plan.dense, workspace, s);
   if (M <= SAMFAST_I4_FEW_ROWS && N >= 16) return launch_i4_few(a, dtype == SAMFAST_F16, s);
   if (plan.splits > 1) a.parts = reinterpret_cast<float*>(workspace);
   return dtype == SAMFAST_F16 ? launch_i4_tiled<ElemF16>(a, plan, s) : launch_i4_tiled<ElemBf16>(a, plan, s);

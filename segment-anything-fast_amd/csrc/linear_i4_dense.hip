@@ -1,55 +1,74 @@
-// Linears with 4-bit weights over many rows where the half types' product by turns (gemm_pingpong.hpp) fits: the weights are written out in the
-// element type, once per call, and that product reads them out of the caches.
+// Linears with 4-bit weights over many rows by the half types' product by turns (gemm_pingpong.hpp): the weights are written out in the
+// element type, once per call, and that product reads them out of the caches.  It walks K by whole 64s: of rows that end inside one, and of their weights, copies
+// with zeros behind them are made.
 #include "gemm_pingpong.hpp"
 #include "linear_i4_shared.hpp"
 
 namespace samfast {
 
-// w[n, k] = (code - zero) * scale, rounded to the element type: eight codes a thread
+static inline int i4_padded(int K) { return (K + 63) / 64 * 64; }
+
+// w[n, k] = (code - zero) * scale, rounded to the element type: eight codes a thread.  Behind N rows of weights, with `copies`, those of x.
 template <class T>
-__global__ __launch_bounds__(256) void i4_weights_kernel(I4Args a, unsigned short* w) {
-  const unsigned int words = (unsigned int)a.K / 8u;  // of a row
+__global__ __launch_bounds__(256) void i4_weights_kernel(I4Args a, unsigned short* w, int padded, int copies) {
+  const unsigned int words = (unsigned int)padded / 8u;  // of a row
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)a.N * words) return;
-  const int n = (int)(i / words), k = 8 * (int)(i - (int64_t)n * words);
+  const int64_t row = i / words;
+  const int k = 8 * (int)(i - row * words);
+  if (row >= a.N || k >= a.K) {
+    u32x4 v = {};
+    if (row >= (int64_t)a.N + copies) return;
+    if (row >= a.N && k < a.K) v = *reinterpret_cast<const u32x4*>(a.x + (row - a.N) * a.ldx + k);
+    reinterpret_cast<u32x4*>(w)[i] = v;
+    return;
+  }
+  const int n = (int)row;
   const int64_t at = (int64_t)(k / a.group) * a.N + n;
   const float s = T::from_bits(a.scales[at]), z = a.zeros ? (float)a.zeros[at] : 8.f;
   float c[8];
-  i4_codes(reinterpret_cast<const unsigned int*>(a.codes)[i], c);
+  i4_codes(reinterpret_cast<const unsigned int*>(a.codes)[row * (a.K / 8) + k / 8], c);
   u32x4 o;
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] = T::pack2((c[2 * e] - z) * s, (c[2 * e + 1] - z) * s);
   reinterpret_cast<u32x4*>(w)[i] = o;
 }
 
-// The time: a launch, the weights read and written, and pp_choose's cost, a unit of which takes 0.085 us where the GPU is nearly idle and 0.115 where it is
-// busy throughout (power).  2048 x 4096 -> 4096 72 us, 4096 x 1280 -> 5120 50, 65536 x 1280 -> 3840 479, 1024 x 8192 -> 8192 153.
+// The time: two launches, weights and copies written and read, and pp_choose's cost, a unit of which takes 0.075 us where the GPU is nearly idle and 0.112 where
+// it is busy throughout (power); 29 shapes lie within a tenth of it, most.  2048 x 4096 -> 4096 72 us, 4096 x 1280 -> 5120 50, 1288 values 53, 65536 x 1280 -> 3840 479,
+// 1024 x 8192 -> 8192 146, 5405 x 3832 -> 4828 177 (copies 17 of it).
 int i4_dense_tile(int64_t M, int N, int K, double* time) {
-  if (K % 64 != 0 || K < 320 || N % 8 != 0 || M < 256 || !launchable((int64_t)N * (K / 8) / 256 + 1, 256)) return 0;
-  const PPChoice c = pp_choose(M, N, K / 64, false, 8.1);
+  const int padded = i4_padded(K);
+  if (padded < 320 || M < 256 || N >= 1 << 22 || !launchable(((int64_t)N + M) * (padded / 8) / 256 + 1, 256)) return 0;
+  const PPChoice c = pp_choose(M, N, padded / 64, false, 8.1);
   if (c.tn == 0) return 0;
   const double fragments = c.tn == 10 ? 12.5 : c.tn == 8 ? 10.0 : 8.1;
-  *time = 4.0 + 2.5 * (double)N * K / 5e6 + (0.085 + 0.03 * c.used) * (double)c.rounds * fragments * (K / 64 + 8);
+  *time = 7.0 + (0.55 * N + (padded != K ? 0.57 * M : 0.0)) * padded / 1e6 + (0.075 + 0.037 * c.used) * (double)c.rounds * fragments * (padded / 64 + 8);
   return c.tn;
+}
+
+int64_t i4_dense_workspace(int64_t M, int N, int K) {
+  const int padded = i4_padded(K);
+  return 2 * (int64_t)padded * (N + (padded != K ? M : 0));
 }
 
 template <class T, class E>
 static int go_dense(const I4Args& a, int tile, unsigned short* weights, hipStream_t stream) {
-  const int64_t words = (int64_t)a.N * (a.K / 8);
-  hipLaunchKernelGGL(i4_weights_kernel<T>, dim3((unsigned int)((words + 255) / 256)), dim3(256), 0, stream, a, weights);
+  const int padded = i4_padded(a.K), copies = padded != a.K ? a.M : 0;
+  const int64_t words = ((int64_t)a.N + copies) * (padded / 8);
+  hipLaunchKernelGGL(i4_weights_kernel<T>, dim3((unsigned int)((words + 255) / 256)), dim3(256), 0, stream, a, weights, padded, copies);
   if (const int rc = check_launch("i4_weights_kernel")) return rc;
   PPArgs p = {};
-  p.x = reinterpret_cast<const unsigned char*>(a.x);
+  p.x = reinterpret_cast<const unsigned char*>(copies ? weights + (int64_t)a.N * padded : a.x);
   p.w = reinterpret_cast<const unsigned char*>(weights);
   p.out = a.y;
   p.bias = a.bias;
   p.ldo = a.ldy;
   p.x_kstep = p.w_kstep = 64;
-  p.x_pitch = (unsigned int)(a.ldx * 2);
-  p.w_pitch = (unsigned int)(a.K * 2);
+  p.x_pitch = (unsigned int)((copies ? padded : a.ldx) * 2);
+  p.w_pitch = (unsigned int)(padded * 2);
   p.M = a.M;
   p.N = a.N;
-  p.nk = a.K / 64;
+  p.nk = padded / 64;
   p.group_m = 4;
   p.tiles_m = (a.M + 255) / 256;
   p.tiles_n = (a.N + 32 * tile - 1) / (32 * tile);

@@ -63,6 +63,7 @@ int launch_i4_few(const I4Args& a, bool f16, hipStream_t stream);  // linear_i4_
 // linear_i4_dense.hip: the weights written out once, then the half types' product by turns.  The tile's columns / 32 and about how many us it
 // takes; 0: not this way
 int i4_dense_tile(int64_t M, int N, int K, double* time);
+int64_t i4_dense_workspace(int64_t M, int N, int K);
 int launch_i4_dense(const I4Args& a, bool f16, int tile, void* weights, hipStream_t stream);
 
 }  // namespace samfast

@@ -231,3 +231,46 @@ def test_outs_that_would_be_read_after_they_are_written_are_refused():
     into = x.clone()
     got = ops.norm_residual(into, residual, gate=gate, post=post, pre=pre, out=into)
     assert torch.equal(into, want[0]) and torch.equal(got[1], want[1])
+
+
+def test_recorded_linear_with_copied_rows():
+    """Rows of 1288 values: their copies lie in the recording's own memory, and are made again at each replay."""
+    from samfast_amd import ops
+    x, codes, scales, z, b = _operands(5000, 1288, 3001, 64, True, torch.bfloat16)
+    call = lambda: ops.linear_i4(x, codes, scales, z, b, group_size=64)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call()
+    for seed in range(3):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda"))
+        want = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+def test_copied_rows_beyond_32_bits():
+    from samfast_amd import ops
+    M, K, N = 290000, 8200, 1029  # 4.76e9 bytes of x, and as many of its copies
+    _, codes, scales, z, b = _operands(1, K, N, 128, True, torch.bfloat16)
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, 130943, 130944, 261888, 262144, M - 130, M - 2, M - 1], device="cuda")
+    x[at] = torch.randn((len(at), K), device="cuda").bfloat16()
+    y = ops.linear_i4(x, codes, scales, z, b, group_size=128)
+    check_linear(y[at].contiguous(), x[at].contiguous(), codes, scales, z, b, 128)
+    assert torch.equal(y[M // 2], b.bfloat16()) and torch.equal(y[M - 3], b.bfloat16())
+
+
+def test_tiles_beyond_32_bits():
+    from samfast_amd import _lib, ops
+    M, K, N = 290000, 8192, 100
+    assert _lib.load().samfast_linear_i4_workspace(M, N, K) == 0  # tiles
+    _, codes, scales, z, b = _operands(1, K, N, 128, True, torch.bfloat16)
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 131071, 131072, 262143, 262144, M - 1], device="cuda")
+    x[at] = torch.randn((len(at), K), device="cuda").bfloat16()
+    y = ops.linear_i4(x, codes, scales, z, b, group_size=128)
+    check_linear(y[at].contiguous(), x[at].contiguous(), codes, scales, z, b, 128)
+    assert torch.equal(y[M // 2], b.bfloat16())

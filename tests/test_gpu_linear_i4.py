@@ -134,3 +134,38 @@ def test_rows_far_apart(M):
     assert torch.equal(ops.linear_i4(prompts[:, -1], codes, scales, z, b, group_size=64), want)
     with ops.record_launches():
         assert torch.equal(ops.linear_i4(prompts[:, -1:], codes, scales, z, b, group_size=64), want.view(M, 1, 96))
+
+
+# rows that end inside 64 values are copied beside the weights, and any number of columns, the last tile over the one before it
+@pytest.mark.parametrize("M,K,N,group,zeros", [(5000, 1288, 3001, 64, True), (3001, 1336, 5121, 32, False), (2500, 2048, 4003, 128, True), (6000, 4000, 1990, 256, True),
+                                               (20000, 400, 2046, 32, True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_written_weights_of_any_shape(M, K, N, group, zeros, dtype):
+    from samfast_amd import _lib, ops
+    padded = -(-K // 64) * 64
+    assert _lib.load().samfast_linear_i4_workspace(M, N, K) == 2 * padded * (N + (M if padded != K else 0))  # this way, not another
+    x, codes, scales, z, b = _operands(M, K, N, group, zeros, dtype)
+    wide = torch.full((M, K + 24), float("nan"), dtype=dtype, device="cuda")
+    wide[:, :K] = x
+    got = ops.linear_i4(wide[:, :K], codes, scales, z, b, group_size=group)
+    _check(got, x, codes, scales, z, b, group)
+    assert torch.equal(ops.linear_i4(x, codes, scales, z, b, group_size=group), got)
+    x[5, K - 1], x[M - 1, 0] = float("inf"), float("nan")
+    odd = ops.linear_i4(x, codes, scales, z, b, group_size=group)
+    rows = torch.ones(M, dtype=torch.bool, device="cuda")
+    rows[5] = rows[M - 1] = False
+    assert torch.equal(odd[rows], got[rows]) and odd[M - 1].isnan().all() and not odd[5].isfinite().any()
+
+
+def test_written_weights_leave_neighbouring_memory_alone():
+    from samfast_amd import _lib, ops
+    lib = _lib.load()
+    for M, K, N in [(5000, 1288, 3001), (2500, 2048, 4003), (3001, 1336, 5121)]:
+        x, codes, scales, z, b = _operands(M, K, N, 32, True, torch.bfloat16)
+        buf = torch.full((M + 2, N + 5), 7.0, dtype=torch.bfloat16, device="cuda")
+        work = torch.empty(lib.samfast_linear_i4_workspace(M, N, K) + 64, dtype=torch.uint8, device="cuda")
+        work[-64:] = 9
+        _lib.check(lib.samfast_linear_i4(x.data_ptr(), K, codes.data_ptr(), scales.data_ptr(), z.data_ptr(), b.data_ptr(), buf[1:].data_ptr(), N + 5,
+                                         work.data_ptr(), M, N, K, 32, 0, torch.cuda.current_stream().cuda_stream), "linear_i4")
+        assert torch.equal(buf[1:M + 1, :N], ops.linear_i4(x, codes, scales, z, b, group_size=32))
+        assert (buf[0] == 7).all() and (buf[M + 1] == 7).all() and (buf[:, N:] == 7).all() and (work[-64:] == 9).all()
