@@ -154,7 +154,7 @@ __global__ __launch_bounds__(1024) void norm_residual_kernel(NormResidualArgs a)
     float* p = part[round++];  // (a place of its own for each of the four sums: no barrier behind the reading)
     if ((lane & 31) == 0) p[half] = v;
     __syncthreads();
-    return half_sum((lane & 31) < a.halves ? p[mine * a.halves + (lane & 31)] : 0.f);
+    return half_sum(!idle && (lane & 31) < a.halves ? p[mine * a.halves + (lane & 31)] : 0.f);  // (an idle half may have no place of its own)
   };
   // f = the row's values; scaled to mean 0 (LayerNorm) and mean square 1, times weights(j) plus weights(j + 1)
   float f[NCH][E];

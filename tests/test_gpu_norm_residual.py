@@ -143,3 +143,18 @@ def test_refusals():
         args = dict(dict(x=x, residual=residual, gate=gate, post=post, pre=pre), **case)
         with pytest.raises(RuntimeError, match="samfast"):
             ops.norm_residual(**args)
+
+
+@pytest.mark.parametrize("K", [4104, 4360, 7935, 7936, 8200])  # 17, 18, 31, 31 halves of wavefronts to a row; 17 with two pieces a thread
+@pytest.mark.parametrize("rms", [False, True])
+def test_rows_of_odd_halves_of_wavefronts(K, rms):
+    """An odd number of halves above 15 leaves half a wavefront without a row; all four sums are taken."""
+    from samfast_amd import ops
+    x, residual, gate, (post, pre) = _inputs(4, K, torch.float16, torch.float32, 2)
+    total, normed = ops.norm_residual(x, residual, gate=gate, post=post, pre=pre, rms=rms)
+    ref_total, ref_normed = _reference(x, residual, gate, post, pre, rms, 1.0, 1.0)
+    _close(total, ref_total, 256 * 2.0 ** -24)
+    spread = (ref_total.abs().amax(-1) / (ref_total.square().mean(-1) if rms else ref_total.var(-1, correction=0)).add(pre[2]).sqrt()).max()
+    _close(normed, ref_normed, 256 * 2.0 ** -24 * max(1.0, float(spread)))
+    again = ops.norm_residual(x, residual, gate=gate, post=post, pre=pre, rms=rms)
+    assert torch.equal(again[0], total) and torch.equal(again[1], normed)
