@@ -265,7 +265,8 @@ extern "C" int samfast_norm_residual(const void* x, int64_t ldx, const void* res
   SF_REQUIRE(post_eps >= 0.f && pre_eps >= 0.f, "norm_residual: eps must not be negative");
   SF_REQUIRE(M == 0 || (x && residual && total), "norm_residual: null pointer");
   SF_REQUIRE(ldx >= K && ld_res >= K, "norm_residual: row strides must hold a row");
-  SF_REQUIRE(M <= 1 || ((total != residual || ld_res == K) && (total != x || (ldx == K && !residual_is_f32))),
+  // (of one row the stride is nothing, but an fp32 total over it still reaches values that other threads have to read)
+  SF_REQUIRE(M == 0 || ((total != residual || M == 1 || ld_res == K) && (total != x || ((M == 1 || ldx == K) && !residual_is_f32))),
              "norm_residual: total lies where its rows are read in another layout");
   if (M == 0) return SAMFAST_OK;
   NormResidualArgs a = {};

@@ -90,3 +90,8 @@ def test_norm_residual_refuses_a_total_over_rows_of_another_layout(change):
 
 def test_rotary_refuses_in_place_in_another_layout():
     _refused(_rotary(), "another layout")
+
+
+def test_norm_residual_refuses_an_fp32_total_over_a_single_half_type_row():
+    _refused(_norm(M=1, total=Q, x=Q, f32=1), "another layout")
+    _refused(_norm(M=1, total=Q, x=Q, residual=Q, f32=1), "another layout")
