@@ -748,9 +748,12 @@ def linear_i4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     N, K = codes.shape[0], 2 * codes.shape[1]
     if N == 0 or K == 0 or K % 8 != 0 or group_size <= 0 or group_size % 32 != 0:
         raise RuntimeError(f"samfast: linear_i4 needs K % 8 == 0 and groups of a multiple of 32 inputs, got K={K}, group_size={group_size}")
+    if N >= 1 << 30 or K > 1 << 20:
+        raise RuntimeError(f"samfast: linear_i4 takes fewer than 2^30 outputs and up to 2^20 inputs, got {N} and {K}")
     if x.dim() == 0 or x.shape[-1] != K:
         raise RuntimeError(f"samfast: linear_i4 needs rows of {K} values, got {tuple(x.shape)}")
     groups = -(-K // group_size)
+    group_size = min(group_size, 1 << 30)  # (one group all the same; its size is a 32-bit argument)
     if tuple(scales.shape) != (groups, N) or scales.dtype != x.dtype or not scales.is_contiguous():
         raise RuntimeError(f"samfast: linear_i4 scales must be a contiguous ({groups}, {N}) tensor of x's dtype")
     if zeros is not None and (tuple(zeros.shape) != (groups, N) or zeros.dtype != torch.uint8 or not zeros.is_contiguous()):
@@ -811,6 +814,8 @@ def norm_residual(x: torch.Tensor, residual: torch.Tensor, *, gate: Optional[tor
     if x.dim() == 0 or x.shape[-1] == 0 or residual.shape != x.shape or residual.dtype not in (x.dtype, torch.float32):
         raise RuntimeError("samfast: norm_residual needs rows, and a residual of x's shape in x's dtype or fp32")
     K = x.shape[-1]
+    if K > 32768:
+        raise RuntimeError(f"samfast: norm_residual takes rows of up to 32768 values, got {K}")
     M = x.numel() // K
     gates = 1
     if gate is not None:
@@ -858,6 +863,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], *k.shape[2:]) != (q.shape[0], *q.shape[2:]))):
         raise RuntimeError("samfast: rotary needs q (B, nH, T, hd) and k (B, nKV, T, hd) of one dtype")
     B, H, T, D = q.shape
+    if D > 1024 or H > 1 << 20 or (k is not None and k.shape[1] > 1 << 20):
+        raise RuntimeError("samfast: rotary takes heads of up to 1024 channels, and up to 2^20 of them")
     if frequencies.dtype != torch.float64 or frequencies.dim() not in (1, 2) or frequencies.numel() == 0 or not frequencies.is_contiguous():
         raise RuntimeError("samfast: rotary frequencies must be a contiguous fp64 (pairs,) or (axes, pairs) tensor")
     axes, pairs = (1, frequencies.shape[0]) if frequencies.dim() == 1 else tuple(frequencies.shape)

@@ -169,3 +169,15 @@ def test_written_weights_leave_neighbouring_memory_alone():
                                          work.data_ptr(), M, N, K, 32, 0, torch.cuda.current_stream().cuda_stream), "linear_i4")
         assert torch.equal(buf[1:M + 1, :N], ops.linear_i4(x, codes, scales, z, b, group_size=32))
         assert (buf[0] == 7).all() and (buf[M + 1] == 7).all() and (buf[:, N:] == 7).all() and (work[-64:] == 9).all()
+
+
+@pytest.mark.parametrize("M", [3, 40, 3000])
+def test_a_group_longer_than_the_rows(M):
+    """One group, however long it is said to be."""
+    from samfast_amd import ops
+    x, codes, scales, z, b = _operands(M, 1000, 520, 1024, True, torch.bfloat16)
+    want = ops.linear_i4(x, codes, scales, z, b, group_size=1024)
+    for group in (1 << 16, (1 << 31) - 32, 1 << 31, (1 << 32) + 32):
+        assert torch.equal(ops.linear_i4(x, codes, scales, z, b, group_size=group), want)
+    with pytest.raises(RuntimeError, match="samfast"):
+        ops.linear_i4(x, codes, scales, z, b, group_size=(1 << 32) + 16)
