@@ -128,7 +128,8 @@ __global__ __launch_bounds__(64 * COLS * SIDES, 2) void linear_i4_kernel(I4Args 
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{};
   const bool one_group = a.group % 128 == 0;  // for a whole k tile
-  auto multiply = [&](const Weights& w, int stage) __attribute__((always_inline)) {
+  // (`left`: inputs from the k tile's first on.  Weights behind the last one are zeros: a zero point times a scale may overflow where no weight does)
+  auto multiply = [&](const Weights& w, int stage, int left = 128) __attribute__((always_inline)) {
     u32x4 x[2][MT], f[4][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) x[0][i] = x_piece(stage, i, 0);
@@ -145,7 +146,10 @@ __global__ __launch_bounds__(64 * COLS * SIDES, 2) void linear_i4_kernel(I4Args 
         for (int t = 0; t < 4; ++t) of[t] = (unsigned int)__builtin_amdgcn_ds_bpermute(4 * (16 * t + lr), (int)sz);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) f[t][j] = i4_weights(T{}, c[t], T::from_bits((unsigned short)of[t]), (float)(of[t] >> 24));
+      for (int t = 0; t < 4; ++t) {
+        f[t][j] = i4_weights(T{}, c[t], T::from_bits((unsigned short)of[t]), (float)(of[t] >> 24));
+        if (32 * t + 8 * lq >= left) f[t][j] = u32x4{};
+      }
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -197,7 +201,7 @@ __global__ __launch_bounds__(64 * COLS * SIDES, 2) void linear_i4_kernel(I4Args 
   if (whole < end && (whole - first) % SIDES == side) {  // its rows were requested with the others
     Weights last;
     load_w_careful(last, whole);
-    multiply(last, (whole - first) / SIDES % 2);
+    multiply(last, (whole - first) / SIDES % 2, a.K - 128 * whole);
   }
   if constexpr (SIDES == 2) {
     meet();

@@ -181,3 +181,21 @@ def test_a_group_longer_than_the_rows(M):
         assert torch.equal(ops.linear_i4(x, codes, scales, z, b, group_size=group), want)
     with pytest.raises(RuntimeError, match="samfast"):
         ops.linear_i4(x, codes, scales, z, b, group_size=(1 << 32) + 16)
+
+
+@pytest.mark.parametrize("K", [1000, 1096, 328])  # the last 128 inputs are not all there
+@pytest.mark.parametrize("M,N", [(3, 131), (40, 131), (300, 200), (5000, 600), (7, 5)])
+@pytest.mark.parametrize("zero", [None, 15, 255])
+def test_scales_that_a_zero_point_carries_beyond_fp16(M, N, K, zero):
+    """Every weight is finite; a scale times its zero point is not."""
+    from samfast_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(M + K)
+    centre = 8 if zero is None else min(zero, 15)
+    low = torch.randint(centre - 2, min(centre + 1, 15) + 1, (N, K), generator=g, device="cuda", dtype=torch.uint8)
+    codes = low[:, 0::2] | low[:, 1::2] << 4
+    groups = -(-K // 64)
+    scales = ((258.0 if zero == 255 else 12000.0) * (1.0 + 0.03 * torch.rand((groups, N), generator=g, device="cuda"))).half()
+    z = None if zero is None else torch.full((groups, N), zero, dtype=torch.uint8, device="cuda")
+    assert scales.double().max() * (8 if zero is None else zero) > 65504 and _weight(codes, scales, z, 64).abs().max() < 65504
+    x = (torch.randn((M, K), generator=g, device="cuda") * 2.0 ** -12).half()
+    _check(ops.linear_i4(x, codes, scales, z, None, group_size=64), x, codes, scales, z, None, 64)
