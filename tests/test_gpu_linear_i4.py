@@ -199,3 +199,18 @@ def test_scales_that_a_zero_point_carries_beyond_fp16(M, N, K, zero):
     assert scales.double().max() * (8 if zero is None else zero) > 65504 and _weight(codes, scales, z, 64).abs().max() < 65504
     x = (torch.randn((M, K), generator=g, device="cuda") * 2.0 ** -12).half()
     _check(ops.linear_i4(x, codes, scales, z, None, group_size=64), x, codes, scales, z, None, 64)
+
+
+@pytest.mark.parametrize("M,K,N", [(3, 1000, 131), (40, 1000, 131), (64, 4096, 200), (300, 1024, 200), (5000, 640, 600), (7, 512, 5)])
+@pytest.mark.parametrize("group", [32, 128])
+def test_scales_that_a_zero_point_carries_beyond_bf16(M, K, N, group):
+    """Weights of at most 7e37 around zero points of 15: fifteen times a scale is more than the type, and fp32, can hold."""
+    from samfast_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(M + K)
+    low = torch.randint(13, 16, (N, K), generator=g, device="cuda", dtype=torch.uint8)
+    codes = low[:, 0::2] | low[:, 1::2] << 4
+    groups = -(-K // group)
+    scales = (2.5e37 * (1.0 + 0.3 * torch.rand((groups, N), generator=g, device="cuda"))).bfloat16()
+    z = torch.full((groups, N), 15, dtype=torch.uint8, device="cuda")
+    x = (torch.randn((M, K), generator=g, device="cuda") * 2.0 ** -20).bfloat16()
+    _check(ops.linear_i4(x, codes, scales, z, None, group_size=group), x, codes, scales, z, None, group)
