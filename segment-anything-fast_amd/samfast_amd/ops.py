@@ -10,6 +10,7 @@ import math
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -684,6 +685,36 @@ def _require_here(name: str, *tensors: Optional[torch.Tensor]) -> None:
             raise RuntimeError(f"samfast: {name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
+# linear_i4, norm_residual and rotary as operators for those who watch a call (tracers, transforms, modes, tensors that are more than their memory), to whom
+# a launch on raw pointers would leave an empty tensor: the same kernels, shapes for tensors without memory, and no derivatives.
+_block_operators = torch.library.Library("samfast", "FRAGMENT")
+
+
+def _register(schema: str, launch, shapes) -> None:
+    name = schema[:schema.index("(")]
+    _block_operators.define(schema)
+
+    def refuse_derivatives(*args):
+        for t in args:
+            if isinstance(t, torch.Tensor) and ((t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None):
+                raise RuntimeError(f"samfast: {name} has no derivatives: call it under torch.no_grad() or on detached tensors")
+        with torch._C._AutoDispatchBelowAutograd():
+            return getattr(torch.ops.samfast, name)(*args)
+
+    _block_operators.impl(name, refuse_derivatives, "Autograd")
+    _block_operators.impl(name, launch, "CUDA")  # (the key of HIP tensors as well)
+    _block_operators.impl(name, shapes, "Meta")
+
+
+def _watched(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether somebody but the kernels has to see a call on these tensors, which then goes to the operator that is registered."""
+    plain = _lib.host().plain
+    if all(t is None or plain(t) for t in tensors):
+        return False
+    _require_gpu(*tensors)
+    return True
+
+
 def _span(t: torch.Tensor) -> Tuple[int, int]:
     """First byte and the byte behind the last that a tensor's elements lie in."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
@@ -736,11 +767,18 @@ def linear_i4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     """Linear with 4-bit weights on half-type rows x (..., K): y = x w^T + bias with w[n, k] = (code[n, k] - zeros[g, n]) * scales[g, n],
     g = k // group_size.  codes: uint8 (N, K/2), the even k in the lower half of a byte; scales (groups, N) of x's dtype; zeros uint8 (groups, N),
     or None for 8; bias fp32 (N).  K a multiple of 8 up to 2^20, group_size of 32; the last group may be shorter.  fp32 sums; up to 32 rows of x (of 16
-    outputs or more) the weights are exact, over more they are rounded to x's dtype.  Returns (..., N)."""
+    outputs or more) the weights are exact, over more they are rounded to x's dtype, and have to be finite in it.  Returns (..., N).
+    Tracers, transforms and modes see torch.ops.samfast.linear_i4; there are no derivatives."""
     if _launch_log is None:
         y = (_lib._host or _lib.host()).linear_i4(x, codes, scales, zeros, bias, group_size)
         if y is not None:
             return y
+    if _watched(x, codes, scales, zeros, bias):
+        return torch.ops.samfast.linear_i4(x, codes, scales, zeros, bias, group_size)
+    return _linear_i4(x, codes, scales, zeros, bias, group_size)
+
+
+def _linear_i4(x, codes, scales, zeros, bias, group_size):
     _require_here("linear_i4", x, codes, scales, zeros, bias)
     dtype = _dtype_code(x)
     if codes.dtype != torch.uint8 or codes.dim() != 2 or not codes.is_contiguous():
@@ -781,6 +819,10 @@ def linear_i4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     return y
 
 
+_register("linear_i4(Tensor x, Tensor codes, Tensor scales, Tensor? zeros, Tensor? bias, int group_size) -> Tensor", _linear_i4,
+          lambda x, codes, scales, zeros, bias, group_size: x.new_empty((*x.shape[:-1], codes.shape[0])))
+
+
 def _norm_weights(name: str, norm, x: torch.Tensor):
     """(gamma, beta, eps) of a norm given as (gamma, beta or None, eps), or of None."""
     if norm is None:
@@ -802,13 +844,25 @@ def norm_residual(x: torch.Tensor, residual: torch.Tensor, *, gate: Optional[tor
     over the last axis of half-type rows x (..., K <= 32768).  post and pre: (gamma, beta or None, eps) of a LayerNorm, or with `rms` of an RMS
     norm, or None to leave it out (normed is then None).  residual: x's shape, x's dtype or fp32; total has its type.  gate: (K), or (G, K) with a
     row for each of G equal runs of x's rows.  fp32 inside; pre sees the total before it is rounded.  `out`: where total goes: the
-    residual itself (or x, of the same type), or memory of its own.  Returns (total, normed)."""
+    residual itself (or x, of the same type), or memory of its own.  Returns (total, normed).  Watched, it is
+    torch.ops.samfast.norm_residual; there are no derivatives."""
     if out is None and _launch_log is None:
         both = (_lib._host or _lib.host()).norm_residual(x, residual, gate, post, pre, rms, branch_scale, residual_scale)
         if both is not None:
             return both
-    post_gamma, post_beta, post_eps = _norm_weights("post", post, x)
-    pre_gamma, pre_beta, pre_eps = _norm_weights("pre", pre, x)
+    weights = (*_norm_weights("post", post, x), *_norm_weights("pre", pre, x))
+    if _watched(x, residual, gate, *weights[:2], *weights[3:5], out):
+        both = torch.ops.samfast.norm_residual(x, residual, gate, *weights, bool(rms), float(branch_scale), float(residual_scale))
+        if out is not None:
+            if out.shape != x.shape or out.dtype != residual.dtype:
+                raise RuntimeError("samfast: out must be a contiguous tensor of the residual's shape and dtype")
+            both[0] = out.copy_(both[0])
+    else:
+        both = _norm_residual(x, residual, gate, *weights, rms, branch_scale, residual_scale, out)
+    return both[0], both[1] if pre is not None else None
+
+
+def _norm_residual(x, residual, gate, post_gamma, post_beta, post_eps, pre_gamma, pre_beta, pre_eps, rms, branch_scale, residual_scale, out=None):
     _require_here("norm_residual", x, residual, gate, post_gamma, post_beta, pre_gamma, pre_beta, out)
     dtype = _dtype_code(x)
     if x.dim() == 0 or x.shape[-1] == 0 or residual.shape != x.shape or residual.dtype not in (x.dtype, torch.float32):
@@ -834,17 +888,23 @@ def norm_residual(x: torch.Tensor, residual: torch.Tensor, *, gate: Optional[tor
     if out is not None:
         _check_out("norm_residual", out, (residual, x), (gate, post_gamma, post_beta, pre_gamma, pre_beta))
     total = torch.empty(x.shape, dtype=residual.dtype, device=x.device) if out is None else out
-    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre is not None else None
+    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre_gamma is not None else None
     ptr = lambda t: t.data_ptr() if t is not None else None
     lib = _lib.load()
     code = _timed(
-        "norm_residual", M * K * (2.0 + 2.0 * residual.element_size() + (2.0 if pre is not None else 0.0)), "byte",
+        "norm_residual", M * K * (2.0 + 2.0 * residual.element_size() + (2.0 if normed is not None else 0.0)), "byte",
         lambda: lib.samfast_norm_residual(
             rows.data_ptr(), rows.stride(0) if M > 1 else K, res.data_ptr(), res.stride(0) if M > 1 else K, ptr(gate), gates,
             ptr(post_gamma), ptr(post_beta), post_eps, ptr(pre_gamma), ptr(pre_beta), pre_eps, int(rms),
             float(branch_scale), float(residual_scale), total.data_ptr(), ptr(normed), M, K, dtype, int(residual.dtype == torch.float32), _stream()))
     _lib.check(code, "norm_residual")
-    return total, normed
+    return [total] if normed is None else [total, normed]
+
+
+_register("norm_residual(Tensor x, Tensor residual, Tensor? gate, Tensor? post_gamma, Tensor? post_beta, float post_eps, Tensor? pre_gamma, Tensor? pre_beta, "
+          "float pre_eps, bool rms, float branch_scale, float residual_scale) -> Tensor[]", _norm_residual,
+          lambda x, residual, gate, post_gamma, post_beta, post_eps, pre_gamma, *rest:
+          [residual.new_empty(x.shape)] + ([] if pre_gamma is None else [x.new_empty(x.shape)]))
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor, *, interleaved: bool = False,
@@ -853,11 +913,31 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     types.  positions int64, (B, T) or (T,); frequencies fp64 (pairs,), radians a position.  For a grid positions (..., T, axes) and
     frequencies (axes, pairs), axes <= 64.  Axis after axis, 2 * pairs channels of the head are turned: pairs of neighbours (`interleaved`), or of a channel
     and its like half of the axis's channels on; channels behind the last axis's are copied.  `scale` multiplies what is turned.  Angles are made in 64
-    bits.  Returns (q', k') in q's and k's shapes, laid out token-major (k' is None where k is), or in `out`, whose tensors are q and k themselves or memory of their own.  Head dims up to 1024."""
+    bits.  Returns (q', k') in q's and k's shapes, laid out token-major (k' is None where k is), or in `out`, whose tensors are q and k themselves or memory of their own.  Head dims up to 1024.
+    Watched, it is torch.ops.samfast.rotary; there are no derivatives."""
     if out is None and _launch_log is None:
         both = (_lib._host or _lib.host()).rotary(q, k, positions, frequencies, interleaved, scale)
         if both is not None:
             return both
+    if _watched(q, k, positions, frequencies, *(out or ())):
+        both = torch.ops.samfast.rotary(q, k, positions, frequencies, bool(interleaved), float(scale))
+        if out is not None:
+            for i, t in enumerate(both):
+                if len(out) <= i or out[i] is None or out[i].shape != t.shape or out[i].dtype != t.dtype:
+                    raise RuntimeError("samfast: out must hold tensors of q's and k's shapes and dtype")
+            both = [o.copy_(t) for o, t in zip(out, both)]
+    else:
+        both = _rotary(q, k, positions, frequencies, interleaved, scale, out)
+    return both[0], both[1] if k is not None else None
+
+
+def _token_major(t):
+    """Memory for heads of t's shape (B, heads, T, hd), the heads of a token side by side."""
+    B, H, T, D = t.shape
+    return t.new_empty((B, T, H, D)).permute(0, 2, 1, 3)
+
+
+def _rotary(q, k, positions, frequencies, interleaved, scale, out=None):
     _require_here("rotary", q, k, positions, frequencies, *(out or ()))
     dtype = _dtype_code(q)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], *k.shape[2:]) != (q.shape[0], *q.shape[2:]))):
@@ -877,7 +957,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     positions = positions.contiguous()
     tensors = [q] if k is None else [q, k]
     if out is None:
-        outs = [torch.empty((B, T, t.shape[1], D), dtype=t.dtype, device=t.device).permute(0, 2, 1, 3) for t in tensors]
+        outs = [_token_major(t) for t in tensors]
     else:
         outs = list(out[:len(tensors)])
         if len(outs) != len(tensors):
@@ -899,7 +979,11 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
             positions.data_ptr(), 0 if shared else T * axes, frequencies.data_ptr(), B, T, H, k.shape[1] if k is not None else 0, D, pairs, axes,
             int(interleaved), float(scale), (ctypes.c_int64 * 12)(*strides), dtype, _stream()))
     _lib.check(code, "rotary")
-    return outs[0], outs[1] if k is not None else None
+    return outs
+
+
+_register("rotary(Tensor q, Tensor? k, Tensor positions, Tensor frequencies, bool interleaved, float scale) -> Tensor[]", _rotary,
+          lambda q, k, *rest: [_token_major(t) for t in (q, k) if t is not None])
 
 
 def neck_convs(x: torch.Tensor, w1: torch.Tensor, norm, w3: torch.Tensor) -> torch.Tensor:
