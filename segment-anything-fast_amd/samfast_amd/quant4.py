@@ -81,9 +81,9 @@ class Int4Linear(nn.Module):
         return dequantize_weight_int4(self.codes, self.scales, self.zeros, self.group_size)
 
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
-        if prefix + "bias" in state_dict:
+        if prefix + "bias" in state_dict and self.bias_bits is not None:  # (without a bias here it is an entry too many)
             value = state_dict.pop(prefix + "bias")
-            if self.bias_bits is not None and prefix + "bias_bits" not in state_dict:
+            if prefix + "bias_bits" not in state_dict:
                 state_dict[prefix + "bias_bits"] = value.detach().to(torch.float32).contiguous().view(torch.int32)
         super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
 

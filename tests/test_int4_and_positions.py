@@ -86,3 +86,19 @@ def test_a_model_is_swapped_whole_or_not_at_all():
     assert [type(m) for m in model] == [torch.nn.Linear, torch.nn.ReLU, torch.nn.Linear]
     apply_int4_weights(model, lambda mod, fqn: fqn == "0")
     assert isinstance(model[0], Int4Linear) and isinstance(model[2], torch.nn.Linear)
+
+
+def test_a_bias_that_the_module_does_not_have_is_not_dropped_silently():
+    from samfast_amd import Int4Linear
+    linear = torch.nn.Linear(64, 40).requires_grad_(False)
+    without = Int4Linear.from_float(torch.nn.Linear(64, 40, bias=False).requires_grad_(False), 32)
+    model = torch.nn.Sequential(without)
+    state = {**model.state_dict(), "0.bias": linear.bias}
+    with pytest.raises(RuntimeError, match="0.bias"):
+        model.load_state_dict(state)
+    assert model.load_state_dict(state, strict=False).unexpected_keys == ["0.bias"] and without.bias is None and "0.bias" in state
+    # one that it has is folded, and not counted as one too many
+    model = torch.nn.Sequential(Int4Linear.from_float(linear, 32))
+    state = {k: v for k, v in model.state_dict().items() if k != "0.bias_bits"}
+    result = model.load_state_dict({**state, "0.bias": linear.bias + 2})
+    assert not result.unexpected_keys and not result.missing_keys and torch.equal(model[0].bias, linear.bias + 2)
