@@ -115,7 +115,7 @@ class Int8LinearBase(nn.Module):
         self.register_buffer("sw_bits", sw.to(torch.float32).contiguous().view(torch.int32))
         if bias is not None:
             self.register_buffer(
-                "bias_bits", bias.detach().to(torch.float32).contiguous().view(torch.int32))
+                "bias_bits", bias.detach().to(torch.float32, copy=True).contiguous().view(torch.int32))
         else:
             self.bias_bits = None
 

@@ -65,7 +65,7 @@ class Int4Linear(nn.Module):
         self.register_buffer("codes", codes)
         self.register_buffer("scales", scales)
         self.register_buffer("zeros", zeros)
-        self.register_buffer("bias_bits", None if bias is None else bias.detach().to(torch.float32).contiguous().view(torch.int32))
+        self.register_buffer("bias_bits", None if bias is None else bias.detach().to(torch.float32, copy=True).contiguous().view(torch.int32))
 
     @classmethod
     def from_float(cls, linear: nn.Linear, group_size: int = 128, zero_points: bool = False) -> "Int4Linear":

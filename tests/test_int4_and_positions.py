@@ -102,3 +102,17 @@ def test_a_bias_that_the_module_does_not_have_is_not_dropped_silently():
     state = {k: v for k, v in model.state_dict().items() if k != "0.bias_bits"}
     result = model.load_state_dict({**state, "0.bias": linear.bias + 2})
     assert not result.unexpected_keys and not result.missing_keys and torch.equal(model[0].bias, linear.bias + 2)
+
+
+@pytest.mark.parametrize("kind", ["Int4Linear", "Int8DynamicLinear"])
+def test_modules_of_one_linear_have_biases_of_their_own(kind):
+    """What is loaded into one of them reaches neither the other nor the Linear."""
+    import samfast_amd
+    make = getattr(samfast_amd, kind).from_float
+    linear = torch.nn.Linear(64, 40).requires_grad_(False)
+    kept = linear.bias.clone()
+    one, other = make(linear), make(linear)
+    one.load_state_dict({**one.state_dict(), "bias_bits": (kept + 1).view(torch.int32)})
+    assert torch.equal(one.bias, kept + 1) and torch.equal(other.bias, kept) and torch.equal(linear.bias, kept)
+    linear.bias += 3
+    assert torch.equal(one.bias, kept + 1) and torch.equal(other.bias, kept)
