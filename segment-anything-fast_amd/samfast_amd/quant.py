@@ -133,9 +133,9 @@ class Int8LinearBase(nn.Module):
 
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
         key = prefix + "bias"
-        if key in state_dict:
+        if key in state_dict and self.bias_bits is not None:  # (without a bias here it is an entry too many)
             value = state_dict.pop(key)
-            if self.bias_bits is not None and prefix + "bias_bits" not in state_dict:
+            if prefix + "bias_bits" not in state_dict:
                 state_dict[prefix + "bias_bits"] = (
                     value.detach().to(torch.float32).contiguous().view(torch.int32))
         super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)

@@ -524,6 +524,15 @@ def test_int8_linear_keeps_one_bias():
     assert Int8DynamicLinear.from_float(nn.Linear(64, 16, bias=False)).bias is None
 
 
+def test_a_bias_that_an_int8_linear_does_not_have_is_reported():
+    from samfast_amd import Int8DynamicLinear
+    model = nn.Sequential(Int8DynamicLinear.from_float(nn.Linear(64, 16, bias=False)))
+    state = {**model.state_dict(), "0.bias": torch.zeros(16)}
+    with pytest.raises(RuntimeError, match="0.bias"):
+        model.load_state_dict(state)
+    assert model.load_state_dict(state, strict=False).unexpected_keys == ["0.bias"] and model[0].bias is None
+
+
 def test_a_block_counts_as_built_only_without_hooks_and_overrides():
     """Only such a block may leave its modules uncalled (the fused half-type route)."""
     from samfast_amd.modeling import Block
