@@ -5,6 +5,7 @@ a quarter of the half types' weight bytes, which is what a step over few rows re
 nothing else, here the weights alone lose bits; the products run in the activations' own type.
 """
 
+import warnings
 from typing import Callable, Optional, Tuple
 
 import torch
@@ -54,7 +55,8 @@ def dequantize_weight_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: Opt
 class Int4Linear(nn.Module):
     """A Linear whose weight is held as `codes`, `scales` and, with zero points, `zeros` (see ops.linear_i4).
 
-    The scales follow the module's dtype, and the kernels compute in it: inputs of another floating type are cast on the way in and the result back.
+    The scales follow the module's dtype between the half types, and the kernels compute in it: inputs of another floating type are cast on the way in and
+    the result back.  A module cast to a wider type keeps them as they are; a cast that takes scales out of the new type's range warns.
     The fp32 bias is kept as int32 bit patterns (`bias_bits`), which no cast of the module rounds; a state dict that carries an nn.Linear's float
     `bias` is folded into it on load.  `weight` is the dequantised weight.  There is no backward pass and no CPU route."""
 
@@ -71,6 +73,18 @@ class Int4Linear(nn.Module):
     def from_float(cls, linear: nn.Linear, group_size: int = 128, zero_points: bool = False) -> "Int4Linear":
         codes, scales, zeros = quantize_weight_int4(linear.weight, group_size, zero_points)
         return cls(linear.in_features, linear.out_features, codes, scales, zeros, linear.bias, group_size)
+
+    def _apply(self, fn, *args, **kwargs):
+        scales = self.scales
+        super()._apply(fn, *args, **kwargs)
+        if self.scales.dtype not in (torch.bfloat16, torch.float16):
+            self.scales = self.scales.to(scales.dtype)  # (there and back is exact)
+        elif self.scales.dtype != scales.dtype and not self.scales.is_meta:
+            scales = scales.to(self.scales.device)
+            lost = (self.scales.isinf() & scales.isfinite()) | ((self.scales == 0) & (scales != 0))
+            if lost.any():
+                warnings.warn(f"{int(lost.sum())} scales of a 4-bit Linear are outside {self.scales.dtype}: their weights are now 0 or not finite", stacklevel=2)
+        return self
 
     @property
     def bias(self) -> Optional[torch.Tensor]:

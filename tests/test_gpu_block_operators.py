@@ -274,3 +274,16 @@ def test_tiles_beyond_32_bits():
     y = ops.linear_i4(x, codes, scales, z, b, group_size=128)
     check_linear(y[at].contiguous(), x[at].contiguous(), codes, scales, z, b, 128)
     assert torch.equal(y[M // 2], b.bfloat16())
+
+
+def test_module_in_an_fp32_model():
+    from samfast_amd import Int4Linear
+    torch.manual_seed(0)
+    module = Int4Linear.from_float(torch.nn.Linear(200, 72).requires_grad_(False), 64, True).to("cuda")
+    x = torch.randn((2, 5, 200), device="cuda")
+    want = module(x)
+    for cast in (module.float, module.double):
+        got = cast()(x)
+        assert got.dtype == torch.float32 and torch.equal(got, want)
+    half = x.bfloat16()
+    check_linear(module(half), half, module.codes, module.scales, module.zeros, module.bias, 64)

@@ -116,3 +116,29 @@ def test_modules_of_one_linear_have_biases_of_their_own(kind):
     assert torch.equal(one.bias, kept + 1) and torch.equal(other.bias, kept) and torch.equal(linear.bias, kept)
     linear.bias += 3
     assert torch.equal(one.bias, kept + 1) and torch.equal(other.bias, kept)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_casts_to_wider_types_keep_the_scales(dtype):
+    """The kernels have half types only; a model in fp32 (or fp64) goes on calling them."""
+    from samfast_amd import Int4Linear
+    torch.manual_seed(1)
+    module = Int4Linear.from_float(torch.nn.Linear(64, 40).to(dtype).requires_grad_(False), 32, True)
+    scales, bias, weight = module.scales.clone(), module.bias.clone(), module.weight.clone()
+    model = torch.nn.Sequential(module, torch.nn.Linear(40, 8))
+    for cast in (model.float, model.double, lambda: model.to(torch.float32)):
+        cast()
+        assert model[1].weight.dtype != dtype
+        assert module.scales.dtype == dtype and torch.equal(module.scales, scales) and torch.equal(module.bias, bias) and torch.equal(module.weight, weight)
+        assert dict(module.named_buffers())["scales"] is module.scales
+
+
+def test_a_cast_that_loses_scales_warns(recwarn):
+    from samfast_amd import Int4Linear
+    linear = torch.nn.Linear(64, 4).to(torch.bfloat16).requires_grad_(False)
+    Int4Linear.from_float(linear, 32).half()
+    assert not recwarn.list
+    for size in (1e-9, 1e7):
+        linear.weight[1] = size
+        with pytest.warns(UserWarning, match="2 scales"):
+            Int4Linear.from_float(linear, 32).half()
