@@ -113,9 +113,9 @@ class Int4Linear(nn.Module):
 def apply_int4_weights(model: nn.Module, filter_fn: Optional[Callable[[nn.Module, str], bool]] = None, group_size: int = 128,
                        zero_points: bool = False) -> None:
     """Swap every nn.Linear under `model` (for which filter_fn(module, fqn) holds, if given) for Int4Linear, in place.  Nothing is swapped where one of them
-    cannot be: inputs that are no multiple of 8."""
+    cannot be: inputs that are no multiple of 8, weights that are not floating-point."""
     chosen = lambda mod, fqn: isinstance(mod, nn.Linear) and (filter_fn is None or filter_fn(mod, fqn))
-    for fqn, mod in model.named_modules():
-        if fqn and chosen(mod, fqn) and (mod.in_features % 8 != 0 or mod.weight.numel() == 0):
-            raise ValueError(f"{fqn}: a 4-bit Linear needs a multiple of 8 inputs, got {mod.in_features}")
+    for fqn, mod in model.named_modules(remove_duplicate=False):  # (under each of its names, as the swap goes by them)
+        if fqn and chosen(mod, fqn) and (mod.in_features % 8 != 0 or mod.weight.numel() == 0 or not mod.weight.is_floating_point()):
+            raise ValueError(f"{fqn}: a 4-bit Linear needs a multiple of 8 inputs and a floating-point weight, got {mod.in_features} and {mod.weight.dtype}")
     replace_with_custom_fn_if_matches_filter(model, lambda linear: Int4Linear.from_float(linear, group_size, zero_points), chosen)

@@ -142,3 +142,16 @@ def test_a_cast_that_loses_scales_warns(recwarn):
         linear.weight[1] = size
         with pytest.warns(UserWarning, match="2 scales"):
             Int4Linear.from_float(linear, 32).half()
+
+
+def test_a_linear_of_two_names_is_looked_at_under_each():
+    from samfast_amd import apply_int4_weights
+    shared = torch.nn.Linear(12, 64)
+    model = torch.nn.ModuleDict({"a": shared, "b": torch.nn.Linear(64, 12), "c": shared, "d": torch.nn.Linear(8, 8)})
+    with pytest.raises(ValueError, match="c: "):
+        apply_int4_weights(model, lambda mod, fqn: fqn in "bc")
+    assert all(type(m) is torch.nn.Linear for m in model.values())
+    model["d"].weight = torch.nn.Parameter(torch.zeros(8, 8, dtype=torch.complex64))
+    with pytest.raises(ValueError, match="d: "):
+        apply_int4_weights(model, lambda mod, fqn: fqn in "bd")
+    assert all(type(m) is torch.nn.Linear for m in model.values())
