@@ -313,7 +313,10 @@ static int go_few(const I4Args& a, hipStream_t stream) {
 }
 template <class T>
 static int go_few(const I4Args& a, hipStream_t stream) {
-  const bool wide = a.N >= 8192;
+  // One workgroup fits a CU (LDS).  32 columns each where 16 would need a second round of the 256 CUs: M x 8192 -> N, groups of 128, us with 16 / 32 columns,
+  // M = 1, 16, 24: N = 4096 7.8 / 10.1, 9.1 / 11.4, 11.1 / 13.6; 5120 11.5 / 10.5, 13.4 / 11.5, 19.1 / 13.7; 8192 11.7 / 10.7, 13.6 / 12.1, 19.5 / 14.2; 16384
+  // 19.5 / 16.9, 22.6 / 18.7, 36.5 / 25.7 (in a recording).  Of three rounds against two up to 16 rows are level, in groups of 32 they lose: 16 x 8192 -> 10240 20.3 / 23.0.
+  const bool wide = a.N > 16 * 256;
   if (a.M <= 16) return wide ? go_few<T, 1, 2>(a, stream) : go_few<T, 1, 1>(a, stream);
   return wide ? go_few<T, 2, 2>(a, stream) : go_few<T, 2, 1>(a, stream);
 }

@@ -98,3 +98,12 @@ def test_one_input_a_row(M, K, N, group, zeros, dtype):
     # at most four fp32 steps: a group's sum scaled and added, the zeros' part scaled and added
     slack = 4 * 2.0 ** -24 * size
     assert ((got - ref).abs() <= slack + half * (ref.abs() + slack) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("M,K,group", [(1, 1000, 32), (16, 512, 128), (24, 2312, 64)])
+@pytest.mark.parametrize("N", [4095, 4096, 4097, 5000, 8191, 8192])
+def test_outputs_around_a_round_of_workgroups(M, K, group, N):
+    """16 or 32 columns to a workgroup, the last columns over the ones before them."""
+    from samfast_amd import ops
+    x, codes, scales, z, b = _operands(M, K, N, group, True, torch.bfloat16)
+    _check_exactly(ops.linear_i4(x, codes, scales, z, b, group_size=group), x, codes, scales, z, b, group)
