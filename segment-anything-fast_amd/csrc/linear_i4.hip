@@ -45,7 +45,10 @@ SF_DEVICE u32x4 i4_weights(ElemF16, unsigned int w, float scale, float zero) {
 
 // Tiles of 16 MT rows and 16 NT COLS columns, K 128 at a time.  The rows of x are everybody's and go through LDS, one k tile ahead; the columns are
 // one wavefront's each, so that a weight is made once in the workgroup and never leaves the registers.  With two SIDES as many wavefronts again take
-// every other k tile, and the sides' sums meet in LDS.  (x and weights two k tiles ahead were level: 512 x 8192 x 8192 77 / 78 us.)
+// every other k tile, and the sides' sums meet in LDS.  (x and weights two k tiles ahead were level.)
+//
+// Making the weights bounds it: at 512 x 4096 -> 4096 vector instructions take 60 % of the SIMDs' cycles, matrix instructions 24 %, LDS reads 25 % of the
+// CUs' cycles, without bank conflicts.
 template <int MT, int NT, int COLS, int SIDES>
 struct I4Tile {
   static constexpr int BM = 16 * MT, BN = 16 * NT * COLS, STAGE = BM * 256, THREADS = 64 * COLS * SIDES;
@@ -305,14 +308,15 @@ __global__ __launch_bounds__(256) void i4_sum_kernel(I4Args a, int splits) {
 }
 
 // How a product is done, from its sizes alone (the workspace is asked for before the call): what takes least by these estimates in us, which lie within
-// a fifth of the times measured.
-//   tiles: 4 + a k tile's time x k tiles x tiles to a CU, alone on it / not; + 3 and the sums' bytes at 6 TB/s where K is split.  Measured, 32 x 64 / 64 x 64 /
-//     128 x 128 tiles: 128 x 1280 -> 3840 7.0 / 8.5 / 12, 333 x 1000 -> 1003 7.5 / 8.8 / 12, 256 x 4096 -> 4096 23.5 / 20.9 / 23 (K split), 512 x 4096 -> 4096
-//     - / 31.2 / 33, 1024 x 1280 -> 3840 - / 22.3 / 18.0, 8000 x 4096 -> 3001 - / 262 / 242; K whole / in four: 64 x 4096 -> 4096 20 / 11.9, 64 x 8192 -> 8192 35 / 20.9,
-//     256 x 4096 -> 4096 20.9 / 24.
-//   dense (linear_i4_dense.hip): by its own estimate.  tiles / dense: 4096 x 1280 -> 5120 73 / 50, 5405 x 3832 -> 4828 267 / 180, 8000 x 4096 -> 3001 242 / 157,
-//     4096 x 1280 -> 5121 84 / 57, 10000 x 328 -> 4001 63 / 49, 1024 x 8192 -> 8192 162 / 146, but 1024 x 4096 -> 4096 50 / 65, 512 x 8192 -> 8192 92 / 128, 4096 x 1280 -> 1280 26 / 28.
-// Up to SAMFAST_I4_FEW_ROWS rows linear_i4_few.hip: 24 x 4096 -> 4096 7.7, tiles 15.
+// a fifth of the times measured, most within a tenth.  Measured in bf16, groups of 128 with zeros, calls that follow one another:
+//   tiles: 4 + a k tile's time x k tiles x tiles to a CU, alone on it / not; + 3 and the sums' bytes at 6 TB/s where K is split.  32 x 64 / 64 x 64 /
+//     128 x 128 tiles: 128 x 1280 -> 3840 7.7 / 8.8 / 17.6, 333 x 1000 -> 1003 7.4 / 8.6 / 15.6, 256 x 4096 -> 4096 24.9 / 20.3 / 23.8 (K in four), 512 x 4096 -> 4096
+//     42 / 30.3 / 34 (K in four), 1024 x 1280 -> 3840 30 / 23.2 / 19.2, 1024 x 4096 -> 4096 79 / 58 / 47; 64 x 64 tiles, K whole / in four: 64 x 4096 -> 4096 20 / 12.1,
+//     64 x 8192 -> 8192 36 / 21.5, 256 x 4096 -> 4096 20.3 / 25.5.
+//   dense (linear_i4_dense.hip): by its own estimate.  128 x 128 tiles / dense: 4096 x 1280 -> 5120 72 / 52, 5405 x 3832 -> 4828 266 / 181, 8000 x 4096 -> 3001 239 / 160,
+//     4096 x 1280 -> 5121 88 / 58, 10000 x 328 -> 4001 69 / 56, 2048 x 4096 -> 4096 82 / 71, 16384 x 1000 -> 1003 53 / 46, but 1024 x 4096 -> 4096 50 / 64, 512 x 8192 -> 8192
+//     92 / 140, 4096 x 1280 -> 1280 26.7 / 27.3; 1024 x 8192 -> 8192 157 / 168 on one card and 162 / 146 on another (the second is taken).
+// Up to SAMFAST_I4_FEW_ROWS rows linear_i4_few.hip: 24 x 4096 -> 4096 7.1, tiles with K in four 10.0.
 struct I4Plan {
   int dense;   // columns / 32 of the dense product's tile, or 0
   int tile;    // 32 x 64, 64 x 64, 128 x 128
@@ -339,7 +343,7 @@ static I4Plan i4_plan(int64_t M, int N, int K) {
     }
   double dense = 0.0;
   const int columns = i4_dense_tile(M, N, K, &dense);
-  // (against the dense product the estimate of the largest tiles is too short: their ends, and the power limit from a round of them on; 16384 x 1000 -> 1003 52, 36 above)
+  // (against the dense product the estimate of the largest tiles is too short: their ends, and the power limit from a round of them on; 16384 x 1000 -> 1003 53, 36 above)
   if (p.tile == 2) least = 1.18 * (least - 4.0) + 4.0 + 2.0 * fmax((double)((M + 127) / 128) * ((N + 127) / 128) / 256.0 - 1.0, 0.0);
   if (columns && dense < least) p = I4Plan{columns, 0, 1};
   return p;

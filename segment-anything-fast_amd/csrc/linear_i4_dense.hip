@@ -34,8 +34,8 @@ __global__ __launch_bounds__(256) void i4_weights_kernel(I4Args a, unsigned shor
 }
 
 // The time: two launches, weights and copies written and read, and pp_choose's cost, a unit of which takes 0.075 us where the GPU is nearly idle and 0.112 where
-// it is busy throughout (power); 29 shapes lie within a tenth of it, most.  2048 x 4096 -> 4096 72 us, 4096 x 1280 -> 5120 50, 1288 values 53, 65536 x 1280 -> 3840 479,
-// 1024 x 8192 -> 8192 146, 5405 x 3832 -> 4828 177 (copies 17 of it).
+// it is busy throughout (power).  2048 x 4096 -> 4096 71 us, 4096 x 1280 -> 5120 52, of 1288 values 54.6, 65536 x 1280 -> 3840 478, 1024 x 8192 -> 8192 146 to 168
+// from card to card, 5405 x 3832 -> 4828 181 (copies 17 of it).
 int i4_dense_tile(int64_t M, int N, int K, double* time) {
   const int padded = i4_padded(K);
   if (padded < 320 || M < 256 || N >= 1 << 22 || !launchable(((int64_t)N + M) * (padded / 8) / 256 + 1, 256)) return 0;

@@ -5,8 +5,9 @@
 // multiplies 32 adjacent k, which belong to one group.  The codes are exact in either type; a group's sum is scaled in fp32, and its zero times the
 // group's sum of x taken off in fp32, so no weight is rounded.  The wavefronts' sums meet in LDS.
 //
-// us (a copy's time for the weights): 1 x 4096 -> 4096 5.1 (1.7), 1 x 8192 -> 8192 9.2 (6.7), with zeros and groups of 32 11.9 (7.7); 24 rows of the last 16.4: 100 MB of x out of the
-// L2s, a workgroup's own rows for each, and about 500 vector instructions for 256 k of two fragments of columns.
+// us, calls that follow one another (a copy's time for the weights): 1 x 4096 -> 4096 5.2 (1.7), 1 x 8192 -> 8192 9.5 (6.7), with zeros and groups of 32 11.9
+// (7.7); 24 rows of the last 16.3 to 16.7.  There 1.2 million lines of 128 bytes come out of the L2s, two thirds of them x, a workgroup's own rows for each; vector
+// instructions, 380 for 256 k of two fragments of columns, take a third of the SIMDs' cycles, matrix instructions 23 %, and wavefronts, two to a SIMD, wait for 37 % of theirs.
 #include "linear_i4_shared.hpp"
 
 #include <type_traits>
@@ -38,7 +39,7 @@ SF_DEVICE u32x4 i4_numbers(unsigned int w) {
 // A wavefront takes 256 k at a time, and the next ones are under way while it multiplies.  The rows of x go straight into LDS of its own, whole lines
 // to a load, and from there into registers: fragments straight from memory are half lines, and 24 x 8192 x 8192 took 22 us instead of 14.  (Codes
 // as fragments or as lines were level.)  Scales and zeros come four columns of a group to a lane, and are handed round by way of LDS: as each lane's own,
-// a load for each group, groups of 32 took 19.6 us instead of 18.0 there (16.4 now).  The loop has no branches, and addresses are uniform bases with 32-bit offsets that are made once: with a K that
+// a load for each group, groups of 32 took 19.6 us instead of 18.0 there (16.5 now).  The loop has no branches, and addresses are uniform bases with 32-bit offsets that are made once: with a K that
 // may end anywhere inside it, the loads of all paths were waited for at each step, and 1 x 8192 x 8192 took 16 us instead of 11.  What is left of K goes
 // through a loop of its own.
 constexpr int kI4FewWaves = 8;
